@@ -64,7 +64,14 @@ enum {
     KH_DTYPE_FLOAT16 = 9,   /* Dtype::Float16 (ordinal in the reference enum) */
     KH_DTYPE_FLOAT32 = 10,  /* Dtype::Float32 */
     KH_DTYPE_BFLOAT16 = 12, /* Dtype::Bfloat16 */
-    KH_DTYPE_FP8_E4M3FN = 100 /* KV-cache only; the reference's native cache format (BM/components/gqa/fp8.rs) */
+    KH_DTYPE_FP8_E4M3FN = 100, /* KV-cache only; the reference's native cache format (BM/components/gqa/fp8.rs) */
+    /* KV-cache only, no reference counterpart: 8-bit codes with a power-of-two scale for every (token, KV head) row.
+     * A page holds [K/V][Hkv][P][D] code bytes and behind them [Hkv][K/V][P] scale bytes b, so page_bytes =
+     * 2 * Hkv * P * (D + 1). A row stands for code * 2^(b - 127); b = 0 marks a row of zeros, and b = 255 a token
+     * whose K or V row (of that KV head) held a NaN or an infinity: both rows then hold zero codes, read back as NaN
+     * and give NaN to every query that sees the token. Head dimensions 128 and 256, pages of 8, 16 or 32 tokens. */
+    KH_DTYPE_INT8_SCALED = 101,      /* two's complement codes in [-127, 127] */
+    KH_DTYPE_FP8_E4M3FN_SCALED = 102 /* FP8 E4M3FN codes, the row's largest magnitude in (224, 448] */
 };
 
 /* ---- device, buffers, streams (stand in for BM/metal/{device,buffer,stream}) --------------- */
@@ -329,10 +336,13 @@ KH_API kh_status kh_metadata_update(const kh_metadata_arrays* arrays, const uint
 /* ---- SlicedKv compute: BM/components/gqa/sdpa/sliced_kv.rs ---------------------------------- */
 /* sliced_kv::Config (sliced_kv.rs:90-98) plus the KV-cache element type, which the reference
  * fixes at one byte (sliced_kv.rs:113-125) and this library makes a parameter. tokens per page =
- * page_bytes / (2 * num_kv_heads * head_dim * sizeof(kv_dtype)).
+ * page_bytes / (2 * num_kv_heads * head_dim * sizeof(kv_dtype)); with the scaled 8-bit kinds
+ * page_bytes / (2 * num_kv_heads * (head_dim + 1)).
  * kv_dtype = KH_DTYPE_FP8_E4M3FN: the reference's cache format; codes are decoded on load exactly as
  * metal/gqa_fp8.metal:1-25 does (16-token pages, head_dim 128 or 256). kv_dtype = dtype: the pages hold
- * Q/output-type elements. */
+ * Q/output-type elements. kv_dtype = KH_DTYPE_INT8_SCALED / KH_DTYPE_FP8_E4M3FN_SCALED: codes with a scale byte for
+ * each (token, KV head) row (every (head_dim, tokens_per_page) profile; kv_pages and q 16-byte aligned; the
+ * one-launch map + reduce form is not offered). */
 typedef struct kh_sliced_kv_config {
     uint32_t num_q_heads;
     uint32_t num_kv_heads;
@@ -599,6 +609,40 @@ KH_API kh_status kh_kv_page_write_tokens_per_page(const kh_kv_page_write_config*
 KH_API kh_status kh_kv_page_write_invoke(kh_kv_page_write* compute, kh_stream* stream,
                                          const kh_kv_page_write_shape* shape, const kh_kv_page_write_buffers* buffers,
                                          uint32_t num_active_token_writes, uint32_t page_table_index);
+/* kv_dtype = KH_DTYPE_INT8_SCALED / KH_DTYPE_FP8_E4M3FN_SCALED quantises each row by itself: with a = max |x| over
+ * the row's head_dim elements, the scale is the smallest power of two 2^e, e >= -126, for which a * 2^-e rounds into
+ * the codes' range (below 127.5 for int8, at most 448 for E4M3FN); codes are x * 2^-e rounded to nearest, ties to
+ * even. A write touches its own rows' codes and scale bytes only. Writes of one call must name distinct positions. */
+
+/* ---- KV page read: the inverse of the page write; no reference counterpart -----------------------------------
+ * Gathers cached K and V rows into flat [rows][Hkv][D] arrays of `dtype`: row i is the token at position
+ * flat_token_indices[i] of request slot req_slots[i] (any order, repeats allowed). Pages of every kv_dtype the page
+ * write stores; values are rounded to `dtype` once (nearest even) and saturate at its largest finite value; NaN stays
+ * NaN. A row whose slot, position or page id lies outside the tables is not written and sets the device status word
+ * as a write does. */
+typedef kh_kv_page_write_config kh_kv_page_read_config;
+typedef struct kh_kv_page_read_shape {
+    uint32_t num_total_token_reads;
+    kh_page_table_layout page_table_layout;
+} kh_kv_page_read_shape;
+typedef struct kh_kv_page_read_buffers {
+    kh_buffer_ref pages;
+    kh_buffer_ref flat_k; /* written */
+    kh_buffer_ref flat_v; /* written */
+    kh_buffer_ref req_slots;
+    kh_buffer_ref flat_token_indices;
+    kh_buffer_ref page_ids;
+} kh_kv_page_read_buffers;
+
+typedef struct kh_kv_page_read kh_kv_page_read;
+
+KH_API kh_status kh_kv_page_read_create(kh_device* device, const kh_kv_page_read_config* config,
+                                        kh_kv_page_read** out);
+KH_API kh_status kh_kv_page_read_destroy(kh_kv_page_read* compute);
+/* Reads the first num_active_token_reads rows; later rows of flat_k / flat_v stay as they are. */
+KH_API kh_status kh_kv_page_read_invoke(kh_kv_page_read* compute, kh_stream* stream,
+                                        const kh_kv_page_read_shape* shape, const kh_kv_page_read_buffers* buffers,
+                                        uint32_t num_active_token_reads, uint32_t page_table_index);
 /* bf16_to_fp8_e4m3 / fp8_e4m3_to_bf16 (BM/components/gqa/fp8.rs:19-58) on bit patterns, host side. */
 KH_API uint8_t kh_fp8_e4m3_from_bf16(uint16_t bf16_bits);
 KH_API uint16_t kh_fp8_e4m3_to_bf16(uint8_t fp8_bits);

@@ -127,6 +127,15 @@ class KvPageWriteBuffersC(C.Structure):
         "pages", "flat_k", "flat_v", "req_slots", "flat_token_indices", "page_ids")]
 
 
+class KvPageReadShapeC(C.Structure):
+    _fields_ = [("num_total_token_reads", C.c_uint32), ("page_table_layout", PageTableLayoutC)]
+
+
+class KvPageReadBuffersC(C.Structure):
+    _fields_ = [(name, BufferRef) for name in (
+        "pages", "flat_k", "flat_v", "req_slots", "flat_token_indices", "page_ids")]
+
+
 class SlicedKvStaticBuffersC(C.Structure):
     _fields_ = [(name, BufferRef) for name in (
         "q", "kv_pages", "req_slots", "page_ids", "sdpa_map_task_templates", "cu_sdpa_partial_outputs", "output")]
@@ -277,6 +286,9 @@ PROTOTYPES = {
     "kh_kv_page_write_destroy": [_vp],
     "kh_kv_page_write_tokens_per_page": [P(KvPageWriteConfigC), P(C.c_uint32)],
     "kh_kv_page_write_invoke": [_vp, _vp, P(KvPageWriteShapeC), P(KvPageWriteBuffersC), _u32, _u32],
+    "kh_kv_page_read_create": [_vp, P(KvPageWriteConfigC), P(_vp)],
+    "kh_kv_page_read_destroy": [_vp],
+    "kh_kv_page_read_invoke": [_vp, _vp, P(KvPageReadShapeC), P(KvPageReadBuffersC), _u32, _u32],
     "kh_combine_packed_partials": [_vp, _vp, _u32, _u32, _u32, BufferRef, _u32, BufferRef],
     "kh_peer_exchange_inbox_bytes": [_u32, _u32, _u32, P(C.c_uint64)],
     "kh_ipc_export": [_vp, BufferRef, P(C.c_uint8)],

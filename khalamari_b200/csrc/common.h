@@ -74,10 +74,29 @@ inline uint32_t dtype_size(kh_dtype dtype) {
         case KH_DTYPE_FLOAT32:
             return 4;
         case KH_DTYPE_FP8_E4M3FN:
+        case KH_DTYPE_INT8_SCALED:
+        case KH_DTYPE_FP8_E4M3FN_SCALED:
             return 1;
         default:
             return 0;
     }
+}
+
+// Pages of 8-bit codes with a scale byte per (token, KV head) row.
+inline bool is_scaled(kh_dtype kv_dtype) {
+    return kv_dtype == KH_DTYPE_INT8_SCALED || kv_dtype == KH_DTYPE_FP8_E4M3FN_SCALED;
+}
+
+// Bytes a page spends on one K or V row.
+inline uint64_t kv_row_bytes(kh_dtype kv_dtype, uint32_t head_dim) {
+    return uint64_t(head_dim) * dtype_size(kv_dtype) + (is_scaled(kv_dtype) ? 1 : 0);
+}
+
+// What the kernels of scaled pages are built for (16-byte code rows, 8-byte groups of scale bytes).
+inline void require_scaled_profile(uint32_t head_dim, uint32_t tokens_per_page) {
+    KH_REQUIRE(head_dim == 128 || head_dim == 256, "scaled 8-bit pages: head_dim 128 and 256 only (got %u)", head_dim);
+    KH_REQUIRE(tokens_per_page == 8 || tokens_per_page == 16 || tokens_per_page == 32,
+               "scaled 8-bit pages hold 8, 16 or 32 tokens (got %u)", tokens_per_page);
 }
 
 }  // namespace kh

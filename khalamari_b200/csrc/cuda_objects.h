@@ -41,6 +41,9 @@ inline void use_device(const kh_device* device) {
     KH_CUDA(cudaSetDevice(device->ordinal));
 }
 
+// Checks a page write / page read configuration and returns its tokens per page (kv_page_write.cu).
+uint32_t page_write_tokens_per_page(const kh_kv_page_write_config& config);
+
 inline void need(kh_buffer_ref buffer, uint64_t bytes, const char* name) {
     KH_REQUIRE(buffer.ptr != nullptr, "%s buffer is null", name);
     KH_REQUIRE(buffer.bytes >= bytes, "%s buffer holds %llu bytes but %llu are required", name,

@@ -14,6 +14,7 @@
 #include <memory>
 
 #include "cuda_objects.h"
+#include "scaled_kv.cuh"
 
 namespace kh {
 
@@ -204,6 +205,106 @@ __global__ void __launch_bounds__(256) kv_page_write_scalar_kernel(const PageWri
     }
 }
 
+// Scaled 8-bit pages (scaled_kv.cuh): a warp quantises the K and V rows of one (write, KV head). At D = 128 lanes 0-15
+// hold the K row and lanes 16-31 the V row, eight elements each; at D = 256 a lane holds eight elements of both. The
+// row maximum is taken over the magnitude bits (ordered as integers; an all-ones exponent or more means a NaN or an
+// infinity), so no value is rounded before its code. HBM-bound: 4 D bytes in, 2 (D + 1) out per row pair.
+template <int CODE, int D>
+__global__ void __launch_bounds__(256) scaled_page_write_kernel(const PageWriteParams p) {
+    constexpr int kPlanes = D / 128;  // planes a lane holds: one at D = 128, K and V at 256
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t heads = p.num_kv_heads;
+    const uint64_t units = uint64_t(p.num_active_token_writes) * heads;
+    const uint32_t infinity = p.source_is_f16 ? 0x7c00u : 0x7f80u;
+    for (uint64_t unit = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; unit < units;
+         unit += (uint64_t(gridDim.x) * blockDim.x) >> 5) {
+        const uint32_t write = uint32_t(unit / heads);
+        const uint32_t head = uint32_t(unit % heads);
+        const uint64_t flat = unit * D + (lane % (D / 8)) * 8;
+        const uint32_t first_plane = kPlanes == 1 ? lane / 16 : 0;
+        uint4 raw[kPlanes];
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) {
+            raw[i] = *reinterpret_cast<const uint4*>((first_plane + i == 0 ? p.flat_k : p.flat_v) + flat);
+        }
+        const uint32_t slot = p.req_slots[write];
+        const uint32_t token = p.flat_token_indices[write];
+        const uint32_t block = token / (p.tokens_per_page * p.num_page_ids_per_block);
+        const uint32_t id_in_block = (token / p.tokens_per_page) % p.num_page_ids_per_block;
+        if (slot >= p.num_req_slots || block >= p.num_blocks) {  // metadata that points past the page table
+            if (lane == 0) atomicOr(p.status, 4u);
+            continue;
+        }
+        const uint64_t entry =
+            ((uint64_t(slot) * p.num_gqa_layers + p.layer_index) * p.num_blocks + block) * p.num_page_ids_per_block +
+            id_in_block;
+        const uint32_t page = p.page_ids[entry];
+        if (page >= p.pool_pages) {  // never write outside the pool; report through the device status word
+            if (lane == 0) atomicOr(p.status, 2u);
+            continue;
+        }
+        uint8_t* const page_base = p.pages + uint64_t(page) * p.page_bytes;
+        const uint32_t row = token % p.tokens_per_page;
+        uint32_t top[kPlanes];
+        bool broken = false;
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) {
+            // per-halfword maximum of the magnitude bits over the row's lanes
+            uint32_t most = __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu),
+                                     __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu));
+#pragma unroll
+            for (int d = (D == 128 ? 8 : 16); d >= 1; d >>= 1) most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, d));
+            top[i] = max(most & 0xffffu, most >> 16);
+            broken = broken || top[i] >= infinity;
+        }
+        broken = __any_sync(0xffffffffu, broken);
+#pragma unroll
+        for (int i = 0; i < kPlanes; ++i) {
+            const uint32_t plane = first_plane + i;
+            const uint16_t top_bits = uint16_t(top[i]);
+            const float largest = p.source_is_f16 ? __half2float(__ushort_as_half(top_bits)) : f32_from_bf16_bits(top_bits);
+            const uint32_t b = broken ? 255u : scale_byte_of<CODE>(largest);
+            const float inverse = __uint_as_float((254u - min(b, 253u)) << 23);  // 2^-e (b <= 249 for finite rows)
+            const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+            float x[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint16_t bits = uint16_t(words[j / 2] >> (16 * (j & 1)));
+                x[j] = p.source_is_f16 ? __half2float(__ushort_as_half(bits)) : f32_from_bf16_bits(bits);
+            }
+            const uint2 codes = b == 0 || broken ? make_uint2(0u, 0u) : encode8<CODE>(x, inverse);
+            const uint64_t at = ((uint64_t(plane) * heads + head) * p.tokens_per_page + row) * D + (lane % (D / 8)) * 8;
+            *reinterpret_cast<uint2*>(page_base + at) = codes;
+            if (lane % (D / 8) == 0) {
+                const uint64_t scales = uint64_t(2) * heads * p.tokens_per_page * D;
+                page_base[scales + (uint64_t(head) * 2 + plane) * p.tokens_per_page + row] = uint8_t(b);
+            }
+        }
+    }
+}
+
+template <int CODE>
+static void launch_scaled_write(const PageWriteParams& p, uint32_t blocks, cudaStream_t stream) {
+    if (p.head_dim == 128) scaled_page_write_kernel<CODE, 128><<<blocks, 256, 0, stream>>>(p);
+    else scaled_page_write_kernel<CODE, 256><<<blocks, 256, 0, stream>>>(p);
+}
+
+// Config::validate + num_tokens_per_page (kv_page_write.rs:69-92), with the stored element size a parameter.
+uint32_t page_write_tokens_per_page(const kh_kv_page_write_config& c) {
+    KH_REQUIRE(c.num_kv_heads > 0 && c.head_dim > 0, "GQA KV page write needs KV heads and a head dimension");
+    KH_REQUIRE(c.dtype == KH_DTYPE_BFLOAT16 || c.dtype == KH_DTYPE_FLOAT16,
+               "GQA KV page write requires BF16 (or FP16) source tensors");
+    KH_REQUIRE(c.kv_dtype == KH_DTYPE_FP8_E4M3FN || c.kv_dtype == c.dtype || is_scaled(c.kv_dtype),
+               "GQA KV pages hold FP8 E4M3FN, scaled 8-bit codes or the source element type");
+    const uint64_t per_token = mul_u64(uint64_t(c.num_kv_heads) * 2, kv_row_bytes(c.kv_dtype, c.head_dim), "GQA K/V bytes per token");
+    KH_REQUIRE(per_token <= 0xffffffffull, "GQA K/V bytes per token must fit u32");
+    KH_REQUIRE(c.page_bytes % per_token == 0, "GQA page_bytes must be divisible by the K/V bytes per token");
+    KH_REQUIRE(c.page_bytes / per_token > 0, "GQA pages must hold at least one token");
+    const uint32_t tokens = uint32_t(c.page_bytes / per_token);
+    if (is_scaled(c.kv_dtype)) require_scaled_profile(c.head_dim, tokens);
+    return tokens;
+}
+
 }  // namespace kh
 
 using namespace kh;
@@ -213,20 +314,6 @@ struct kh_kv_page_write {
     kh_kv_page_write_config config;
     uint32_t tokens_per_page;
 };
-
-// Config::validate + num_tokens_per_page (kv_page_write.rs:69-92), with the stored element size a parameter.
-static uint32_t page_write_tokens_per_page(const kh_kv_page_write_config& c) {
-    KH_REQUIRE(c.num_kv_heads > 0 && c.head_dim > 0, "GQA KV page write needs KV heads and a head dimension");
-    KH_REQUIRE(c.dtype == KH_DTYPE_BFLOAT16 || c.dtype == KH_DTYPE_FLOAT16,
-               "GQA KV page write requires BF16 (or FP16) source tensors");
-    KH_REQUIRE(c.kv_dtype == KH_DTYPE_FP8_E4M3FN || c.kv_dtype == c.dtype,
-               "GQA KV pages hold FP8 E4M3FN or the source element type");
-    const uint64_t per_token = uint64_t(c.num_kv_heads) * c.head_dim * 2 * dtype_size(c.kv_dtype);
-    KH_REQUIRE(per_token <= 0xffffffffull, "GQA K/V bytes per token must fit u32");
-    KH_REQUIRE(c.page_bytes % per_token == 0, "GQA page_bytes must be divisible by the K/V bytes per token");
-    KH_REQUIRE(c.page_bytes / per_token > 0, "GQA pages must hold at least one token");
-    return uint32_t(c.page_bytes / per_token);
-}
 
 extern "C" {
 
@@ -313,7 +400,14 @@ kh_status kh_kv_page_write_invoke(kh_kv_page_write* compute, kh_stream* stream, 
             uint64_t(num_active_token_writes) * c.num_kv_heads * (vector ? c.head_dim / 8 : c.head_dim);
         const uint32_t blocks = uint32_t(std::min<uint64_t>((threads + 255) / 256, uint64_t(compute->device->sm_count) * 8));
         const bool fp8 = dtype_size(c.kv_dtype) == 1;
-        if (vector && fp8) kv_page_write_kernel<1><<<blocks, 256, 0, stream->stream>>>(p);
+        if (is_scaled(c.kv_dtype)) {
+            KH_REQUIRE(vector, "scaled 8-bit pages: pages, flat_k and flat_v must be 16-byte aligned");
+            const uint64_t warps = uint64_t(num_active_token_writes) * c.num_kv_heads;
+            const uint32_t scaled_blocks =
+                uint32_t(std::min<uint64_t>((warps + 7) / 8, uint64_t(compute->device->sm_count) * 8));
+            if (c.kv_dtype == KH_DTYPE_INT8_SCALED) launch_scaled_write<kCodeInt8>(p, scaled_blocks, stream->stream);
+            else launch_scaled_write<kCodeE4M3>(p, scaled_blocks, stream->stream);
+        } else if (vector && fp8) kv_page_write_kernel<1><<<blocks, 256, 0, stream->stream>>>(p);
         else if (vector) kv_page_write_kernel<2><<<blocks, 256, 0, stream->stream>>>(p);
         else if (fp8) kv_page_write_scalar_kernel<1><<<blocks, 256, 0, stream->stream>>>(p);
         else kv_page_write_scalar_kernel<2><<<blocks, 256, 0, stream->stream>>>(p);

@@ -17,6 +17,7 @@ struct MapInstance {
     int stage_tokens;
     int box_rows;
     int stages;
+    int rows_per_block = 0;  // scaled pages: Q rows of a task that one work item takes; 0: all of them
 };
 
 // Warp-level instance for K/V pages of FP8 E4M3FN elements (sdpa_fp8.cu; compiled apart from the 16-bit instances
@@ -24,5 +25,8 @@ struct MapInstance {
 // must support the map + reduce in one launch form (arrival counters).
 MapInstance pick_instance_fp8(kh_dtype dtype, uint32_t head_dim, uint32_t tokens_per_page, uint32_t rows,
                               bool one_launch);
+
+// Instance for scaled 8-bit pages (sdpa_scaled.cu).
+MapInstance pick_instance_scaled(kh_dtype dtype, kh_dtype kv_dtype, uint32_t head_dim, uint32_t rows);
 
 }  // namespace kh

@@ -395,7 +395,8 @@ static void init_common(ComputeCommon& c, kh_device* device, kh_dtype dtype, kh_
                         const kh_page_table_layout& layout, const kh_execution_variant& variant) {
     use_device(device);
     const bool fp8 = kv_dtype == KH_DTYPE_FP8_E4M3FN;
-    KH_REQUIRE(kv_dtype == dtype || fp8, "K/V pages hold the Q/output element type or FP8 E4M3FN");
+    KH_REQUIRE(kv_dtype == dtype || fp8 || is_scaled(kv_dtype),
+               "K/V pages hold the Q/output element type, FP8 E4M3FN or scaled 8-bit codes");
     c.device = device;
     c.dtype = dtype;
     c.kv_dtype = kv_dtype;
@@ -406,8 +407,15 @@ static void init_common(ComputeCommon& c, kh_device* device, kh_dtype dtype, kh_
     c.page_bytes = page_bytes;
     c.layout = layout;
     c.variant = variant;
-    c.tokens_per_page = page_bytes / (2 * num_kv_heads * head_dim * dtype_size(kv_dtype));
+    c.tokens_per_page = static_cast<uint32_t>(page_bytes / (2 * num_kv_heads * kv_row_bytes(kv_dtype, head_dim)));
     const uint32_t rows = variant.max_q_tokens * variant.max_q_heads;
+    if (is_scaled(kv_dtype)) {
+        require_scaled_profile(head_dim, c.tokens_per_page);
+        c.instance = pick_instance_scaled(dtype, kv_dtype, head_dim, rows);
+        KH_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(c.instance.kernel),
+                                     cudaFuncAttributeMaxDynamicSharedMemorySize, c.instance.smem_bytes));
+        return;
+    }
     c.instance = fp8 ? pick_instance_fp8(dtype, head_dim, c.tokens_per_page, rows, false)
                      : pick_instance(dtype, head_dim, c.tokens_per_page, rows, true);
     // the one-launch map + reduce form counts arrivals inside the warp-level kernel
@@ -423,8 +431,18 @@ static void launch_map(ComputeCommon& c, kh_stream* stream, MapParams& p, kh_buf
                        uint32_t num_templates) {
     KH_REQUIRE(stream != nullptr && stream->device == c.device, "stream does not belong to the compute's device");
     use_device(c.device);
-    const CUtensorMap& map = c.pool_map(kv_pages);
-    const CUtensorMap& qmap = c.q_map(q);
+    const bool scaled = is_scaled(c.kv_dtype);
+    CUtensorMap unused{};
+    if (scaled) {
+        KH_REQUIRE(p.cu == nullptr, "scaled 8-bit pages: the one-launch map + reduce form is not available");
+        KH_REQUIRE((reinterpret_cast<uintptr_t>(kv_pages.ptr) & 15) == 0, "kv_pages must be 16-byte aligned");
+        KH_REQUIRE((reinterpret_cast<uintptr_t>(q.ptr) & 15) == 0, "q must be 16-byte aligned");
+        p.q = q.ptr;
+        p.kv_pages = static_cast<const uint8_t*>(kv_pages.ptr);
+        p.page_bytes = c.page_bytes;
+    }
+    const CUtensorMap& map = scaled ? unused : c.pool_map(kv_pages);
+    const CUtensorMap& qmap = scaled ? unused : c.q_map(q);
     p.status = c.device->status;
     p.num_templates = num_templates;
     p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
@@ -451,7 +469,10 @@ static void launch_map(ComputeCommon& c, kh_stream* stream, MapParams& p, kh_buf
     }
 #endif
     if (num_templates == 0) return;
-    const uint64_t tasks = uint64_t(num_templates) * c.num_kv_heads * p.head_ranges;
+    uint64_t tasks = uint64_t(num_templates) * c.num_kv_heads * p.head_ranges;
+    if (c.instance.rows_per_block != 0) {
+        tasks *= div_ceil(p.max_q_tokens * p.heads_per_task, uint32_t(c.instance.rows_per_block));
+    }
     KH_REQUIRE(tasks <= 0xffffffffull, "GQA SDPA map task count must fit u32");
     const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(tasks, uint64_t(c.device->sm_count)));
     const MapInstance& instance = p.cu != nullptr ? c.fused_instance : c.instance;
@@ -510,9 +531,8 @@ static uint64_t layout_entries(const kh_page_table_layout& l) {
 }
 
 static uint32_t tokens_per_page_of(uint32_t page_bytes, uint32_t num_kv_heads, uint32_t head_dim, kh_dtype kv_dtype) {
-    const uint32_t elem = dtype_size(kv_dtype);
-    KH_REQUIRE(elem > 0, "unknown K/V element type");
-    const uint64_t per_token = uint64_t(num_kv_heads) * head_dim * 2 * elem;
+    KH_REQUIRE(dtype_size(kv_dtype) > 0, "unknown K/V element type");
+    const uint64_t per_token = mul_u64(uint64_t(num_kv_heads) * 2, kv_row_bytes(kv_dtype, head_dim), "GQA K/V bytes per token");
     KH_REQUIRE(per_token <= 0xffffffffull, "GQA K/V bytes per token must fit u32");
     KH_REQUIRE(page_bytes % per_token == 0, "GQA page_bytes must be divisible by the K/V bytes per token");
     const uint32_t tokens = static_cast<uint32_t>(page_bytes / per_token);

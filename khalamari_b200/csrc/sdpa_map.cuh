@@ -80,6 +80,10 @@ struct MapParams {
     // state from one task to the next (outputs stay valid); 1024 tensor-memory kernel: skip the remainder MMAs;
     // 4096 FP8 pages: the decode warps hand stages on without converting them.
     uint32_t debug;
+    // Scaled 8-bit pages (sdpa_scaled.cuh), which are read through plain addresses:
+    const void* q;
+    const uint8_t* kv_pages;
+    uint32_t page_bytes;
 };
 
 constexpr uint32_t kStatusWaitExpired = 1u;

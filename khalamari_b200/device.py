@@ -18,9 +18,20 @@ class Dtype(enum.IntEnum):
     Float32 = 10
     Bfloat16 = 12
     Fp8E4M3FN = 100
+    # KV-cache pages only, no reference counterpart: 8-bit codes with a power-of-two scale byte per (token, KV head) row
+    Int8Scaled = 101
+    Fp8E4M3Scaled = 102
 
     def item_size(self) -> int:
-        return {Dtype.Uint32: 4, Dtype.Float16: 2, Dtype.Float32: 4, Dtype.Bfloat16: 2, Dtype.Fp8E4M3FN: 1}[self]
+        return {Dtype.Uint32: 4, Dtype.Float16: 2, Dtype.Float32: 4, Dtype.Bfloat16: 2, Dtype.Fp8E4M3FN: 1,
+                Dtype.Int8Scaled: 1, Dtype.Fp8E4M3Scaled: 1}[self]
+
+    def is_scaled(self) -> bool:
+        return self in (Dtype.Int8Scaled, Dtype.Fp8E4M3Scaled)
+
+    def kv_row_bytes(self, head_dim: int) -> int:
+        """Bytes a page of this K/V element type spends on one (token, KV head) row of K or V."""
+        return head_dim * self.item_size() + (1 if self.is_scaled() else 0)
 
 
 class Device:

@@ -42,8 +42,9 @@ class GQAAttention:
                  page_table_layout: GQAPageTableLayout, max_tokens: int,
                  policy: SelectorPolicy = SelectorPolicy.B200, selector: Selector | None = None,
                  kv_dtype: Dtype | None = None):
-        """``kv_dtype``: element type of the K/V pages; ``io_dtype`` (default) or ``Dtype.Fp8E4M3FN``, the
-        reference's cache format (decoded on load, components/gqa/sdpa/sliced_kv.rs:118)."""
+        """``kv_dtype``: element type of the K/V pages; ``io_dtype`` (default), ``Dtype.Fp8E4M3FN``, the
+        reference's cache format (decoded on load, components/gqa/sdpa/sliced_kv.rs:118), or ``Dtype.Int8Scaled`` /
+        ``Dtype.Fp8E4M3Scaled``, 8-bit codes with a scale per (token, KV head) row (two-launch form only)."""
         core.validate()
         self.device = device
         self.core = core
@@ -51,8 +52,7 @@ class GQAAttention:
         self.kv_dtype = io_dtype if kv_dtype is None else kv_dtype
         self.page_bytes = page_bytes
         self.layout = page_table_layout
-        elem = self.kv_dtype.item_size()
-        self.tokens_per_page = page_bytes // (2 * core.num_kv_heads * core.head_dim * elem)
+        self.tokens_per_page = page_bytes // (2 * core.num_kv_heads * self.kv_dtype.kv_row_bytes(core.head_dim))
         self.sdpa_config = sdpa.Config(io_dtype, core.num_q_heads, core.num_kv_heads, core.head_dim,
                                        self.tokens_per_page)
         if selector is None:
