@@ -264,7 +264,9 @@ typedef struct kh_selection kh_selection;
 typedef uint32_t kh_selector_policy;
 enum {
     KH_POLICY_REFERENCE = 0, /* the reference's rules, bit for bit (calibrated for a 40-core Apple GPU) */
-    KH_POLICY_B200 = 1       /* same route table, KV slice re-derived for `sm_count` SMs */
+    KH_POLICY_B200 = 1,      /* same route table, KV slice re-derived for `sm_count` SMs */
+    KH_POLICY_B200_CHAINED = 2 /* KH_POLICY_B200 with decode and verify slices a quarter as long: for map kernels that
+                                * merge neighbouring slices of the same Q rows (scaled 8-bit pages) */
 };
 
 /* Selector::new(Registry::from_variants(config, variants), ...) (sdpa.rs:137-165, sdpa.rs:276-285).
@@ -284,7 +286,7 @@ KH_API kh_status kh_selector_destroy(kh_selector* selector);
 KH_API kh_status kh_selector_limits_get(const kh_selector* selector, kh_selector_limits* out);
 KH_API kh_status kh_selector_variants(const kh_selector* selector, kh_execution_variant* out, uint32_t capacity,
                                       uint32_t* count);
-/* Sets the routing policy and the SM count the KH_POLICY_B200 slice rule targets. */
+/* Sets the routing policy and the SM count the KH_POLICY_B200* slice rules target. */
 KH_API kh_status kh_selector_set_policy(kh_selector* selector, kh_selector_policy policy, uint32_t sm_count);
 
 /* Selector::select (sdpa.rs:278-380). The replay bucket policy is

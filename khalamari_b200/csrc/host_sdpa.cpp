@@ -424,7 +424,7 @@ Route lookup_route_reference(const kh_sdpa_config& c, const kh_request_shape* re
 //    ring busy; 64 for batches too small to give every SM a task) and never above 2048 (bounds the per-task
 //    tail).
 Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* requests, uint32_t num_requests,
-                        uint32_t sm_count) {
+                        uint32_t sm_count, bool chained) {
     // measured: decode (one Q token per task) runs best with about 4 tasks per SM (2,048-token slices on the decode
     // bench and on 1M tokens); Q-tile tasks, fewer and costlier, balance better with about 8
     constexpr uint32_t kTasksPerSm = 8;
@@ -473,8 +473,16 @@ Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* request
             // one task per tile writes the output directly, no partials and no reduce (chunked prefill)
             slice = end;
         } else {
+            // A map kernel that merges neighbouring slices of the same rows before it publishes them pays nothing for
+            // short slices and balances better with them (64 decode sequences over 8-bit pages: 512-token slices
+            // instead of 2,048 leave no SM more than 3 % behind instead of 13 %).
+            const uint32_t finer = chained && variant.max_q_tokens * variant.max_q_heads <= 32 ? 4 : 1;
             slice = decode_slice(end, work * head_groups, min_slice, 2048,
-                                 (unsigned __int128)sm_count * (sliced_q ? kTasksPerSm : kDecodeTasksPerSm));
+                                 (unsigned __int128)sm_count * (sliced_q ? kTasksPerSm : kDecodeTasksPerSm) * finer);
+            if (finer > 1) {
+                // ... and at most 128 slices of one sequence, which is what these kernels divide freely among SMs
+                while (div_ceil(end, slice) > 128) slice *= 2;
+            }
             // A small batch cut at 256 tokens leaves most SMs without a task (four short decode requests with two
             // KV heads: 32 tasks on 148 SMs, and the batch sits in L2, so the step is pure latency). When the tasks
             // at this slice do not reach the SM count, aim at one task per SM and allow slices down to 64 tokens.
@@ -884,11 +892,11 @@ kh_status kh_selector_variants(const kh_selector* selector, kh_execution_variant
 kh_status kh_selector_set_policy(kh_selector* selector, kh_selector_policy policy, uint32_t sm_count) {
     return guarded([&]() -> kh_status {
         KH_REQUIRE(selector != nullptr, "null argument");
-        KH_REQUIRE(policy == KH_POLICY_REFERENCE || policy == KH_POLICY_B200, "unknown selector policy");
+        KH_REQUIRE(policy == KH_POLICY_REFERENCE || policy == KH_POLICY_B200 || policy == KH_POLICY_B200_CHAINED, "unknown selector policy");
         KH_REQUIRE(sm_count > 0, "selector policy requires an SM count");
         selector->policy = policy;
         selector->sm_count = sm_count;
-        if (policy == KH_POLICY_B200 && selector->lookup) {
+        if (policy != KH_POLICY_REFERENCE && selector->lookup) {
             // Make every variant the B200 route can return a member of the registry, so that
             // Selection::variant() always belongs to the selector that produced it.
             const kh_sdpa_config& c = selector->config;
@@ -897,7 +905,7 @@ kh_status kh_selector_set_policy(kh_selector* selector, kh_selector_policy polic
             for (uint32_t queries = 1; queries <= limit; queries *= 2) {
                 for (uint32_t end : {32u, 8192u}) {
                     kh_request_shape probe{end - std::min(end, queries), queries};
-                    const Route route = lookup_route_b200(c, &probe, 1, sm_count);
+                    const Route route = lookup_route_b200(c, &probe, 1, sm_count, policy == KH_POLICY_B200_CHAINED);
                     if (!contains_variant(*selector, route.variant)) selector->variants.push_back(route.variant);
                     max_tile = std::max(max_tile, route.variant.max_q_tokens);
                 }
@@ -926,8 +934,9 @@ kh_status kh_selector_select(const kh_selector* selector, const kh_request_shape
                                num_total_tokens, has_slice, slice, direct);
         };
         if (s.lookup) {
-            Route route = s.policy == KH_POLICY_B200 ? lookup_route_b200(c, requests, num_requests, s.sm_count)
-                                                     : lookup_route_reference(c, requests, num_requests);
+            Route route = s.policy == KH_POLICY_REFERENCE
+                              ? lookup_route_reference(c, requests, num_requests)
+                              : lookup_route_b200(c, requests, num_requests, s.sm_count, s.policy == KH_POLICY_B200_CHAINED);
             if (!route.direct) {
                 // sum ceil(visible / slice) <= ceil(sum_visible / slice) + ranges - 1: coarsen the
                 // slice until the templates fit the initialised capacity (sdpa.rs:290-307).

@@ -27,6 +27,8 @@ MapInstance pick_instance_fp8(kh_dtype dtype, uint32_t head_dim, uint32_t tokens
                               bool one_launch);
 
 // Instance for scaled 8-bit pages (sdpa_scaled.cu).
-MapInstance pick_instance_scaled(kh_dtype dtype, kh_dtype kv_dtype, uint32_t head_dim, uint32_t rows);
+// `paired`: neighbouring KV heads can share a copy (an even number of them, one Q-head range each).
+MapInstance pick_instance_scaled(kh_dtype dtype, kh_dtype kv_dtype, uint32_t head_dim, uint32_t tokens_per_page, uint32_t rows,
+                                 bool paired);
 
 }  // namespace kh

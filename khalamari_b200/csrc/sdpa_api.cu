@@ -49,6 +49,7 @@ struct ReduceParams {
     uint32_t heads_per_block;  // > 1 (one-token ranges only): a block serves this many consecutive heads
     const uint32_t* active;    // replay: device words {tokens, Q-token tiles, templates}; the counts above bound them
     uint32_t active_range_word; // which of the words counts this launch's ranges (0: tokens, 1: Q-token tiles)
+    uint32_t wide;             // long partial lists: the widest block, whose thread groups share a row's list
 };
 
 template <typename T>
@@ -355,7 +356,7 @@ struct ComputeCommon {
 
     const CUtensorMap& pool_map(kh_buffer_ref pages) {
         if (const CUtensorMap* hit = find_map(pool_maps, pages)) return *hit;
-        KH_REQUIRE((reinterpret_cast<uintptr_t>(pages.ptr) & 127) == 0, "kv_pages must be 128-byte aligned");
+        KH_REQUIRE(is_scaled(kv_dtype) || (reinterpret_cast<uintptr_t>(pages.ptr) & 127) == 0, "kv_pages must be 128-byte aligned");
         const uint64_t pool_pages = pages.bytes / page_bytes;
         KH_REQUIRE(pool_pages > 0, "kv_pages holds no complete page");
         const uint64_t rows = pool_pages * 2 * num_kv_heads * tokens_per_page;
@@ -363,6 +364,22 @@ struct ComputeCommon {
         PoolMap entry{};
         entry.ptr = pages.ptr;
         entry.bytes = pages.bytes;
+        if (is_scaled(kv_dtype)) {
+            // Pages end with their scale bytes, so the page is a dimension of its own: {128-byte line, rows of a plane,
+            // lines of a row, K/V plane, page}.
+            const uint64_t plane_rows = uint64_t(num_kv_heads) * tokens_per_page;
+            const cuuint64_t dims[5] = {128, plane_rows, head_dim / 128, 2, pool_pages};
+            const cuuint64_t strides[4] = {head_dim, 128, plane_rows * head_dim, page_bytes};
+            const cuuint32_t box[5] = {128, static_cast<cuuint32_t>(instance.box_rows), head_dim / 128, 2, 1};
+            const cuuint32_t elem_strides[5] = {1, 1, 1, 1, 1};
+            const CUresult rc = encode_tiled_fn()(&entry.map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 5, pages.ptr, dims, strides, box,
+                                                  elem_strides, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+            if (rc != CUDA_SUCCESS) raise(KH_INTERNAL, "cuTensorMapEncodeTiled (scaled pages) failed with code %d", int(rc));
+            if (pool_maps.size() >= kTensorMapCacheEntries) pool_maps.erase(pool_maps.begin());
+            pool_maps.push_back(entry);
+            return pool_maps.back().map;
+        }
         // Four dimensions: {64 columns, pool rows, 64-column halves of a row, K/V plane}. A copy at
         // (0, first K row of a page chunk, 0, 0) with box {64, rows, halves, 2} brings the K chunk and, one
         // plane stride (Hkv * P rows) further, the V chunk of the same (page, KV head). Rows are addressed
@@ -411,7 +428,8 @@ static void init_common(ComputeCommon& c, kh_device* device, kh_dtype dtype, kh_
     const uint32_t rows = variant.max_q_tokens * variant.max_q_heads;
     if (is_scaled(kv_dtype)) {
         require_scaled_profile(head_dim, c.tokens_per_page);
-        c.instance = pick_instance_scaled(dtype, kv_dtype, head_dim, rows);
+        const bool paired = num_kv_heads % 2 == 0 && variant.max_q_heads >= num_q_heads / num_kv_heads && c.tokens_per_page <= 16;
+        c.instance = pick_instance_scaled(dtype, kv_dtype, head_dim, c.tokens_per_page, rows, paired);
         KH_CUDA(cudaFuncSetAttribute(reinterpret_cast<const void*>(c.instance.kernel),
                                      cudaFuncAttributeMaxDynamicSharedMemorySize, c.instance.smem_bytes));
         return;
@@ -437,11 +455,12 @@ static void launch_map(ComputeCommon& c, kh_stream* stream, MapParams& p, kh_buf
         KH_REQUIRE(p.cu == nullptr, "scaled 8-bit pages: the one-launch map + reduce form is not available");
         KH_REQUIRE((reinterpret_cast<uintptr_t>(kv_pages.ptr) & 15) == 0, "kv_pages must be 16-byte aligned");
         KH_REQUIRE((reinterpret_cast<uintptr_t>(q.ptr) & 15) == 0, "q must be 16-byte aligned");
+        KH_REQUIRE(c.page_bytes <= 0x7fffffffu, "scaled 8-bit pages must be smaller than 2 GiB");
         p.q = q.ptr;
         p.kv_pages = static_cast<const uint8_t*>(kv_pages.ptr);
         p.page_bytes = c.page_bytes;
     }
-    const CUtensorMap& map = scaled ? unused : c.pool_map(kv_pages);
+    const CUtensorMap& map = c.pool_map(kv_pages);
     const CUtensorMap& qmap = scaled ? unused : c.q_map(q);
     p.status = c.device->status;
     p.num_templates = num_templates;
@@ -485,7 +504,7 @@ static void launch_reduce_typed(const ReduceParams& p, uint32_t num_ranges, cuda
     ReduceParams params = p;
     dim3 grid(num_ranges, p.num_q_heads, 1);
     // a fixed, long partial list per row (the cross-slice and cross-GPU merges) gets the widest block
-    uint32_t threads = (p.cu == nullptr && p.fixed_partials > 32) ? kReduceMaxThreads : 128;
+    uint32_t threads = (p.cu == nullptr && p.fixed_partials > 32) || p.wide != 0 ? kReduceMaxThreads : 128;
     params.heads_per_block = 1;
     const uint32_t slots = p.head_dim / 4;
     if (p.max_q_tokens == 1 && threads == 128 && slots <= 64 && 128 % slots == 0) {
@@ -517,6 +536,13 @@ static void launch_reduce(kh_dtype dtype, const ReduceParams& p, uint32_t num_ra
     else if (dtype == KH_DTYPE_FLOAT32) launch_reduce_typed<float>(p, num_ranges, stream);
     else raise(KH_INVALID_ARGUMENT, "unsupported output dtype");
     KH_CUDA(cudaGetLastError());
+}
+
+// The map kernels of scaled pages leave one full partial per chain of slices among empty ones, so their lists are long
+// and mostly statistics. From 32 partials per range on, a row's list is shared by the thread groups of a wide block (one
+// sequence of 524,288 tokens in 1,024 slices: the reduce takes 150 us in one list, and a sixteenth of the steps here).
+static uint32_t wide_reduce(kh_dtype kv_dtype, uint32_t templates, uint32_t ranges) {
+    return is_scaled(kv_dtype) && templates / ranges >= 32 ? 1u : 0u;
 }
 
 static void validate_layout(const kh_page_table_layout& l) {
@@ -1142,6 +1168,7 @@ kh_status kh_sliced_kv_reduce(kh_sliced_kv* compute, kh_stream* stream, const kh
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 0;
+        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens);
         launch_reduce(compute->config.dtype, p, num_active_tokens, stream->stream);
         return KH_OK;
     });
@@ -1352,6 +1379,7 @@ kh_status kh_sliced_q_reduce(kh_sliced_q* compute, kh_stream* stream, const kh_s
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 1;
+        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_q_token_tiles);
         launch_reduce(compute->config.dtype, p, num_active_q_token_tiles, stream->stream);
         return KH_OK;
     });

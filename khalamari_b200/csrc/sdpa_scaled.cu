@@ -8,43 +8,59 @@
 
 namespace kh {
 
-template <typename T, int CODE, int D, int NQ, int W>
-static MapInstance make_scaled_instance() {
-    using G = ScaledGeometry<D, NQ, W>;
-    return MapInstance{sdpa_scaled_kernel<T, CODE, D, NQ, W>, G::kThreads, G::kSmemBytes, G::kTileTokens, 0, G::kSlots, G::kRows};
+template <typename T, int CODE, int D, int NQ, int W, int HP, int NT>
+static MapInstance make_stream_instance() {
+    using G = ScaledGeometry<D, NQ, W, HP, true>;
+    return MapInstance{sdpa_scaled_stream_kernel<T, CODE, D, NQ, W, HP, NT>, G::kThreads, G::kSmemBytes, G::kTileTokens, HP * 16,
+                       G::kSlots, G::kRows};
 }
 
-// Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM. Wider tasks are worked on in
-// blocks of rows, which read the KV range again (from L2).
+template <typename T, int CODE, int D, int NQ, int W>
+static MapInstance make_chain_instance() {
+    using G = ScaledGeometry<D, NQ, W, 1, false>;
+    return MapInstance{sdpa_scaled_chain_kernel<T, CODE, D, NQ, W>, G::kThreads, G::kSmemBytes, G::kTileTokens, 16, G::kSlots, G::kRows};
+}
+
+// Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM. Tasks wider than the widest
+// instance are worked on in blocks of rows, which read the KV range again (from L2). `paired`: the KV heads can be taken
+// two at a time.
 template <typename T, int CODE, int D>
-static MapInstance pick_scaled_rows(uint32_t rows) {
+static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {
     if constexpr (D == 128) {
-        if (rows <= 8) return make_scaled_instance<T, CODE, 128, 1, 16>();
-        if (rows <= 16) return make_scaled_instance<T, CODE, 128, 2, 12>();
-        if (rows <= 24) return make_scaled_instance<T, CODE, 128, 3, 8>();
-        return make_scaled_instance<T, CODE, 128, 4, 8>();
+        if (rows <= 8 && paired) return make_stream_instance<T, CODE, 128, 1, 12, 2, 1>();
+        if (rows <= 8) return make_stream_instance<T, CODE, 128, 1, 12, 1, 1>();
+        if (rows <= 16) return make_stream_instance<T, CODE, 128, 2, 8, 1, 1>();
+        if (rows <= 24) return make_chain_instance<T, CODE, 128, 3, 8>();
+        return make_chain_instance<T, CODE, 128, 4, 8>();
     } else {
-        if (rows <= 8) return make_scaled_instance<T, CODE, 256, 1, 8>();
-        if (rows <= 16) return make_scaled_instance<T, CODE, 256, 2, 8>();
-        return make_scaled_instance<T, CODE, 256, 3, 8>();
+        if (rows <= 8) return make_stream_instance<T, CODE, 256, 1, 8, 1, 1>();
+        if (rows <= 16) return make_chain_instance<T, CODE, 256, 2, 8>();
+        return make_chain_instance<T, CODE, 256, 3, 8>();
     }
 }
 
 template <typename T, int CODE>
-static MapInstance pick_scaled_dim(uint32_t head_dim, uint32_t rows) {
-    return head_dim == 128 ? pick_scaled_rows<T, CODE, 128>(rows) : pick_scaled_rows<T, CODE, 256>(rows);
+static MapInstance pick_scaled_dim(uint32_t head_dim, uint32_t rows, bool paired) {
+    return head_dim == 128 ? pick_scaled_rows<T, CODE, 128>(rows, paired) : pick_scaled_rows<T, CODE, 256>(rows, paired);
 }
 
 template <typename T>
-static MapInstance pick_scaled_code(kh_dtype kv_dtype, uint32_t head_dim, uint32_t rows) {
-    return kv_dtype == KH_DTYPE_INT8_SCALED ? pick_scaled_dim<T, kCodeInt8>(head_dim, rows) : pick_scaled_dim<T, kCodeE4M3>(head_dim, rows);
+static MapInstance pick_scaled_code(kh_dtype kv_dtype, uint32_t head_dim, uint32_t rows, bool paired) {
+    return kv_dtype == KH_DTYPE_INT8_SCALED ? pick_scaled_dim<T, kCodeInt8>(head_dim, rows, paired)
+                                            : pick_scaled_dim<T, kCodeE4M3>(head_dim, rows, paired);
 }
 
-MapInstance pick_instance_scaled(kh_dtype dtype, kh_dtype kv_dtype, uint32_t head_dim, uint32_t rows) {
+MapInstance pick_instance_scaled(kh_dtype dtype, kh_dtype kv_dtype, uint32_t head_dim, uint32_t tokens_per_page, uint32_t rows, bool paired) {
     KH_REQUIRE(rows >= 1 && rows <= 128, "a Map task holds at most 128 (Q token, Q head) rows (got %u)", rows);
-    if (dtype == KH_DTYPE_BFLOAT16) return pick_scaled_code<__nv_bfloat16>(kv_dtype, head_dim, rows);
-    KH_REQUIRE(dtype == KH_DTYPE_FLOAT16, "Q/output dtype must be Bfloat16 or Float16 on this backend");
-    return pick_scaled_code<__half>(kv_dtype, head_dim, rows);
+    MapInstance instance;
+    if (dtype == KH_DTYPE_BFLOAT16) {
+        instance = pick_scaled_code<__nv_bfloat16>(kv_dtype, head_dim, rows, paired);
+    } else {
+        KH_REQUIRE(dtype == KH_DTYPE_FLOAT16, "Q/output dtype must be Bfloat16 or Float16 on this backend");
+        instance = pick_scaled_code<__half>(kv_dtype, head_dim, rows, paired);
+    }
+    instance.box_rows = instance.box_rows / 16 * int(tokens_per_page < 16 ? tokens_per_page : 16);
+    return instance;
 }
 
 }  // namespace kh

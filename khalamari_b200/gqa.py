@@ -57,6 +57,8 @@ class GQAAttention:
                                        self.tokens_per_page)
         if selector is None:
             selector = Selector.for_lookup(self.sdpa_config, max_tokens, page_table_layout)
+            if policy == SelectorPolicy.B200 and self.kv_dtype.is_scaled():
+                policy = SelectorPolicy.B200Chained  # what the map kernels of scaled pages do best with
             selector.set_policy(policy, device.sm_count())
         self.selector = selector
         limits = selector.limits()

@@ -16,6 +16,7 @@ from .sdpa import Config, ExecutionVariant, MapKernelKind, Registry
 class SelectorPolicy(enum.IntEnum):
     Reference = 0  # the reference's rules, bit for bit
     B200 = 1       # KV slice and Q tile re-derived for a persistent kernel on `sm_count` SMs
+    B200Chained = 2  # B200 with finer decode / verify slices, for map kernels that merge neighbouring slices
 
 
 @dataclass(frozen=True)
