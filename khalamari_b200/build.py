@@ -18,7 +18,7 @@ LIBRARY = PACKAGE_DIR / "libkhcuda_gqa.so"
 MEASURE_LIBRARY = PACKAGE_DIR / "libkhcuda_gqa_measure.so"
 SOURCES = ["host_sdpa.cpp", "sdpa_api.cu", "sdpa_fp8.cu", "sdpa_scaled.cu", "kv_page_write.cu", "kv_page_read.cu", "bidi_block_sdpa.cu", "peer_exchange.cu"]
 HEADERS = ["common.h", "cuda_objects.h", "host_sdpa.h", "map_instance.h", "sdpa_map.cuh", "sdpa_tc.cuh", "sdpa_tm.cuh",
-           "sdpa_scaled.cuh", "scaled_kv.cuh", "../../include/kh_gqa.h"]
+           "sdpa_scaled.cuh", "sdpa_scaled_tc.cuh", "scaled_kv.cuh", "../../include/kh_gqa.h"]
 
 
 def nvcc_path() -> str:

@@ -537,3 +537,77 @@ def test_prefill_and_decode_in_one_call(device):
     q = Buffer.from_slice(device, case.q_bits)
     mixed.record_sdpa(run.stream, q, run.pages, run.ids, Buffer.wrap(device, run.out.ref.ptr, tokens * run.row * 2))
     assert_close(run.read(), *reference(case))
+
+
+# ---- wide Q tiles -----------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,page,histories,q_lens", [
+    (16, 2, 16, [700, 0, 133], [200, 129, 49]),   # odd numbers of tiles: pairs that straddle two requests
+    (32, 8, 8, [300], [333]),                     # a group of four heads, 32-token tiles
+    (12, 2, 16, [61, 5], [97, 64]),               # a group of six: 96 of 128 rows
+    (8, 1, 16, [2000], [40]),                     # few tiles: the KV range is cut
+    (5, 1, 8, [0], [300]),
+])
+def test_wide_tiles_match_the_64_bit_restatement(device, code, io, hq, hkv, page, histories, q_lens):
+    case = make_scaled_case(hq + page, code, io, hq, hkv, 128, histories, q_lens, page=page)
+    run = ScaledRun(device, case, max_tokens=512)
+    out = run.run()
+    execution = run.attention.metadata.variant().thread_block
+    assert execution.max_q_tokens * execution.max_q_heads > 32
+    assert_close(out, *reference(case))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("io,low,high", [("bf16", -40, 40), ("f16", -14, 11)])
+def test_wide_tiles_over_rows_of_very_different_sizes(device, code, io, low, high):
+    """V rows whose scales differ by up to 2^80 (f16: up to its whole range), some of them zero."""
+    def some_zero(rng, tokens, heads):
+        return _wild(low, high)(rng, tokens, heads) * (rng.random((tokens, heads)) > 0.2)
+    case = make_scaled_case(80, code, io, 16, 2, 128, [200, 0], [64, 80], k_scale=_wild(-6, 1), v_scale=some_zero)
+    assert_close(ScaledRun(device, case, max_tokens=256).run(), *reference(case))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+def test_wide_tiles_and_rows_that_are_not_finite(device, code, io):
+    case = make_scaled_case(81, code, io, 16, 2, 128, [300, 150], [64, 40])
+    codes, scales = planes(case.pool, 2, 16, 128)
+    at = 330  # a token of request 0's own chunk, KV head 1: seen by its queries from number 30 on
+    page = case.table[case.slots[0], 0, at // 16]
+    scales[page, 1, :, at % 16] = 255
+    codes[page, :, 1, at % 16] = 0
+    run = ScaledRun(device, case, max_tokens=256)
+    run.plan()
+    run.record()
+    out = run.read()
+    expected, bound = reference(case)
+    hidden = np.zeros(out.shape[:2], bool)
+    hidden[30:64, 8:] = True
+    assert np.isnan(out[hidden]).all()
+    assert_close(out[~hidden], expected[~hidden], bound[~hidden])
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("page", [8, 16])
+def test_wide_tiles_with_windows(device, code, page):
+    """Direct output with per-token visible ranges: windows of different lengths, empty ones, unallocated pages below."""
+    from khalamari_b200 import sliced_q
+    from khalamari_b200.device import Buffer
+    from khalamari_b200.sdpa import ExecutionVariant
+    hq, hkv, d, tokens, context = 16, 2, 128, 32, 500
+    case = make_scaled_case(82, code, "bf16", hq, hkv, d, [context - tokens], [tokens], page=page)
+    case.table[case.slots[0], 0, :200 // page] = 0xFFFFFF00
+    run = ScaledRun(device, case)
+    config = sliced_q.Config(hq, hkv, d, case.scale, page_bytes(hkv, page, d), run.io, run.layout, run.kv)
+    windows = [(200 + 7 * i, 200 + 7 * i + (0 if i % 5 == 3 else 40 + 3 * i)) for i in range(tokens)]
+    execution = ExecutionVariant.sliced_q(config.sdpa_config(), 3, 16, 16, 8)
+    shape = sliced_q.Shape(tokens, 2, 2)
+    compute = sliced_q.Compute.new_direct(device, config, execution, shape)
+    buffers = [Buffer.from_slice(device, np.array(x, np.uint32)) for x in (
+        [case.slots[0]] * tokens, windows, [(0, 16), (16, 32)], [(0, 0, context), (1, 0, context)])]
+    compute.invoke_direct(run.stream, sliced_q.DirectBuffers(run.q, run.pages, buffers[0], run.ids, *buffers[1:], run.out), 0, tokens, 2)
+    out = run.read()
+    expected, bound = reference(case, [(0, b, e) for b, e in windows])
+    assert_close(out, expected, bound)
+    assert not out[3].any()
