@@ -1,7 +1,9 @@
 // KV page read: gathers cached K and V rows into flat [rows][Hkv][D] arrays, the inverse of the page write
 // (kv_page_write.cu) for every page element type it stores. Addresses as there; scale bytes as in scaled_kv.cuh.
 // HBM-bound: a lane turns eight codes (8 bytes, or 16 of a 16-bit page) into 16 output bytes, so that a warp's loads
-// and stores are whole lines.
+// and stores are whole lines; over scaled pages a warp takes a whole row (all heads), four vectors in flight per lane,
+// which spreads the address arithmetic that bounded a thread-per-vector form (320 us for 117,332 rows of 4 x 256; floor
+// 110 us).
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
@@ -35,23 +37,19 @@ struct PageReadParams {
 };
 
 // What a page stores.
-enum PageKind : int { kPage16 = 0, kPageE4M3 = 1, kPageInt8Scaled = 2, kPageE4M3Scaled = 3 };
+enum PageKind : int { kPage16 = 0, kPageE4M3 = 1 };  // (scaled pages have a kernel of their own)
 
-// Rounded once to T, nearest even, saturating at the largest finite value; NaN stays NaN.
+// E4M3 values are exact in both types.
 template <typename T>
-__device__ __forceinline__ uint32_t pack_saturated(float lo, float hi);
+__device__ __forceinline__ uint32_t pack_exact(float lo, float hi);
 template <>
-__device__ __forceinline__ uint32_t pack_saturated<__half>(float lo, float hi) {
-    // (fminf drops a NaN, so it is put back)
-    const float a = lo != lo ? lo : fminf(fmaxf(lo, -65504.0f), 65504.0f), b = hi != hi ? hi : fminf(fmaxf(hi, -65504.0f), 65504.0f);
-    const __half2 v = __floats2half2_rn(a, b);
+__device__ __forceinline__ uint32_t pack_exact<__half>(float lo, float hi) {
+    const __half2 v = __floats2half2_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 template <>
-__device__ __forceinline__ uint32_t pack_saturated<__nv_bfloat16>(float lo, float hi) {
-    const float most = __uint_as_float(0x7f7f0000u);
-    const float a = lo != lo ? lo : fminf(fmaxf(lo, -most), most), b = hi != hi ? hi : fminf(fmaxf(hi, -most), most);
-    const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+__device__ __forceinline__ uint32_t pack_exact<__nv_bfloat16>(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t*>(&v);
 }
 
@@ -60,7 +58,6 @@ __device__ __forceinline__ uint32_t pack_saturated<__nv_bfloat16>(float lo, floa
 template <typename T, int KIND, int VEC>
 __global__ void __launch_bounds__(256) kv_page_read_kernel(const PageReadParams p) {
     constexpr int kBytes = KIND == kPage16 ? 2 : 1;
-    constexpr int kCode = KIND == kPageInt8Scaled ? kCodeInt8 : kCodeE4M3;
     const uint32_t vecs = p.head_dim / VEC;
     const uint32_t per_read = 2 * p.num_kv_heads * vecs;  // [head][plane][vector]
     const uint64_t total = uint64_t(p.num_active_token_reads) * per_read;
@@ -95,11 +92,6 @@ __global__ void __launch_bounds__(256) kv_page_read_kernel(const PageReadParams 
             if constexpr (VEC == 8) *reinterpret_cast<uint4*>(out) = *reinterpret_cast<const uint4*>(page_base + elem * kBytes);
             else *out = *reinterpret_cast<const uint16_t*>(page_base + elem * kBytes);
         } else {
-            float scale = 1.0f;
-            if constexpr (KIND == kPageInt8Scaled || KIND == kPageE4M3Scaled) {
-                const uint64_t scales = uint64_t(2) * p.num_kv_heads * p.tokens_per_page * p.head_dim;
-                scale = scale_of_byte(page_base[scales + (uint64_t(head) * 2 + plane) * p.tokens_per_page + row]);
-            }
             uint32_t words[(VEC + 3) / 4];
             if constexpr (VEC == 8) {
                 const uint2 raw = *reinterpret_cast<const uint2*>(page_base + elem);
@@ -112,12 +104,12 @@ __global__ void __launch_bounds__(256) kv_page_read_kernel(const PageReadParams 
 #pragma unroll
             for (int w = 0; w < (VEC + 3) / 4; ++w) {
                 uint32_t lo, hi;
-                codes4_to_half<kCode>(words[w], lo, hi);
+                codes4_to_half<kCodeE4M3>(words[w], lo, hi);
                 const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
-                packed[2 * w] = pack_saturated<T>(a.x * scale, a.y * scale);
+                packed[2 * w] = pack_exact<T>(a.x, a.y);
                 if constexpr (VEC == 8) {
                     const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-                    packed[2 * w + 1] = pack_saturated<T>(b.x * scale, b.y * scale);
+                    packed[2 * w + 1] = pack_exact<T>(b.x, b.y);
                 }
             }
             if constexpr (VEC == 8) *reinterpret_cast<uint4*>(out) = make_uint4(packed[0], packed[1], packed[2], packed[3]);
@@ -126,20 +118,87 @@ __global__ void __launch_bounds__(256) kv_page_read_kernel(const PageReadParams 
     }
 }
 
-template <typename T, int KIND>
-static void launch_read(const PageReadParams& p, bool vector, uint32_t blocks, cudaStream_t stream) {
-    if (vector) {
-        kv_page_read_kernel<T, KIND, 8><<<blocks, 256, 0, stream>>>(p);
-    } else {
-        if constexpr (KIND == kPage16 || KIND == kPageE4M3) kv_page_read_kernel<T, KIND, 1><<<blocks, 256, 0, stream>>>(p);
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(256) scaled_page_read_kernel(const PageReadParams p) {
+    constexpr uint32_t kVecs = D / 8;   // vectors of a row
+    constexpr int kFlight = 4;
+    const uint32_t lane = threadIdx.x & 31;
+    const uint32_t heads = p.num_kv_heads, P = p.tokens_per_page;
+    const uint32_t per_plane = heads * kVecs, per_read = 2 * per_plane;
+    for (uint64_t unit = (uint64_t(blockIdx.x) * blockDim.x + threadIdx.x) >> 5; unit < p.num_active_token_reads;
+         unit += (uint64_t(gridDim.x) * blockDim.x) >> 5) {
+        const uint32_t slot = p.req_slots[unit];
+        const uint32_t token = p.flat_token_indices[unit];
+        const uint32_t block = token / (P * p.num_page_ids_per_block);
+        const uint32_t id_in_block = (token / P) % p.num_page_ids_per_block;
+        if (slot >= p.num_req_slots || block >= p.num_blocks) {  // metadata that points past the page table
+            if (lane == 0) atomicOr(p.status, 4u);
+            continue;
+        }
+        const uint64_t entry =
+            ((uint64_t(slot) * p.num_gqa_layers + p.layer_index) * p.num_blocks + block) * p.num_page_ids_per_block +
+            id_in_block;
+        const uint32_t page = p.page_ids[entry];
+        if (page >= p.pool_pages) {
+            if (lane == 0) atomicOr(p.status, 2u);
+            continue;
+        }
+        const uint32_t row = token % P;
+        const uint8_t* const codes = p.pages + uint64_t(page) * p.page_bytes + uint64_t(row) * D;
+        const uint8_t* const scales = p.pages + uint64_t(page) * p.page_bytes + uint64_t(2) * heads * P * D + row;
+        for (uint32_t base = lane; base < per_read; base += 32 * kFlight) {
+            uint2 raw[kFlight];
+            uint32_t b[kFlight];
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i) {
+                const uint32_t vec = base + 32 * i;
+                if (vec < per_read) {
+                    const uint32_t plane = vec >= per_plane ? 1 : 0, line = vec / kVecs, head = line - plane * heads;  // line = plane * heads + head
+                    raw[i] = *reinterpret_cast<const uint2*>(codes + uint64_t(line) * P * D + vec % kVecs * 8);
+                    b[i] = scales[(head * 2 + plane) * P];
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < kFlight; ++i) {
+                const uint32_t vec = base + 32 * i;
+                if (vec < per_read) {
+                    const uint32_t plane = vec >= per_plane ? 1 : 0;
+                    uint32_t one, two, v[4];
+                    scaled_factors<T>(b[i], false, one, two);
+                    decode4<T, CODE>(raw[i].x, one, two, v[0], v[1]);
+                    decode4<T, CODE>(raw[i].y, one, two, v[2], v[3]);
+                    if (b[i] >= first_large_byte<T>()) {
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) v[j] = saturate2<T>(v[j]);
+                    }
+                    uint16_t* const out = (plane == 0 ? p.flat_k : p.flat_v) + (unit * heads * kVecs + (vec - plane * per_plane)) * 8;
+                    *reinterpret_cast<uint4*>(out) = make_uint4(v[0], v[1], v[2], v[3]);
+                }
+            }
+        }
     }
 }
 
+template <typename T, int KIND>
+static void launch_read(const PageReadParams& p, bool vector, uint32_t blocks, cudaStream_t stream) {
+    if (vector) kv_page_read_kernel<T, KIND, 8><<<blocks, 256, 0, stream>>>(p);
+    else kv_page_read_kernel<T, KIND, 1><<<blocks, 256, 0, stream>>>(p);
+}
+
+template <typename T, int CODE>
+static void launch_scaled_read(const PageReadParams& p, uint32_t sm_count, cudaStream_t stream) {
+    const uint32_t blocks = std::min<uint32_t>((p.num_active_token_reads + 7) / 8, sm_count * 64);
+    if (p.head_dim == 128) scaled_page_read_kernel<T, CODE, 128><<<blocks, 256, 0, stream>>>(p);
+    else scaled_page_read_kernel<T, CODE, 256><<<blocks, 256, 0, stream>>>(p);
+}
+
 template <typename T>
-static void launch_read_kind(const PageReadParams& p, kh_dtype kv_dtype, bool vector, uint32_t blocks, cudaStream_t stream) {
-    if (kv_dtype == KH_DTYPE_INT8_SCALED) launch_read<T, kPageInt8Scaled>(p, vector, blocks, stream);
-    else if (kv_dtype == KH_DTYPE_FP8_E4M3FN_SCALED) launch_read<T, kPageE4M3Scaled>(p, vector, blocks, stream);
-    else if (kv_dtype == KH_DTYPE_FP8_E4M3FN) launch_read<T, kPageE4M3>(p, vector, blocks, stream);
+static void launch_read_kind(const PageReadParams& p, kh_dtype kv_dtype, bool vector, uint32_t sm_count, cudaStream_t stream) {
+    if (kv_dtype == KH_DTYPE_INT8_SCALED) return launch_scaled_read<T, kCodeInt8>(p, sm_count, stream);
+    if (kv_dtype == KH_DTYPE_FP8_E4M3FN_SCALED) return launch_scaled_read<T, kCodeE4M3>(p, sm_count, stream);
+    const uint64_t threads = uint64_t(p.num_active_token_reads) * 2 * p.num_kv_heads * (vector ? p.head_dim / 8 : p.head_dim);
+    const uint32_t blocks = uint32_t(std::min<uint64_t>((threads + 255) / 256, uint64_t(sm_count) * 8));
+    if (kv_dtype == KH_DTYPE_FP8_E4M3FN) launch_read<T, kPageE4M3>(p, vector, blocks, stream);
     else launch_read<T, kPage16>(p, vector, blocks, stream);
 }
 
@@ -224,11 +283,8 @@ kh_status kh_kv_page_read_invoke(kh_kv_page_read* compute, kh_stream* stream, co
         p.tokens_per_page = compute->tokens_per_page;
         p.page_bytes = c.page_bytes;
         p.pool_pages = uint32_t(std::min<uint64_t>(buffers->pages.bytes / c.page_bytes, 0xffffffffull));
-        const uint64_t threads =
-            uint64_t(num_active_token_reads) * 2 * c.num_kv_heads * (vector ? c.head_dim / 8 : c.head_dim);
-        const uint32_t blocks = uint32_t(std::min<uint64_t>((threads + 255) / 256, uint64_t(compute->device->sm_count) * 8));
-        if (c.dtype == KH_DTYPE_FLOAT16) launch_read_kind<__half>(p, c.kv_dtype, vector, blocks, stream->stream);
-        else launch_read_kind<__nv_bfloat16>(p, c.kv_dtype, vector, blocks, stream->stream);
+        if (c.dtype == KH_DTYPE_FLOAT16) launch_read_kind<__half>(p, c.kv_dtype, vector, compute->device->sm_count, stream->stream);
+        else launch_read_kind<__nv_bfloat16>(p, c.kv_dtype, vector, compute->device->sm_count, stream->stream);
         KH_CUDA(cudaGetLastError());
         return KH_OK;
     });

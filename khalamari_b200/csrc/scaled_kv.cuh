@@ -12,6 +12,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 namespace kh {
 
@@ -40,8 +41,11 @@ __device__ __forceinline__ uint2 encode8(const float (&x)[8], float inverse) {
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
         if constexpr (CODE == kCodeInt8) {
-            const uint32_t c0 = uint32_t(__float2int_rn(x[4 * w] * inverse)), c1 = uint32_t(__float2int_rn(x[4 * w + 1] * inverse));
-            const uint32_t c2 = uint32_t(__float2int_rn(x[4 * w + 2] * inverse)), c3 = uint32_t(__float2int_rn(x[4 * w + 3] * inverse));
+            // 1.5 * 2^23 has a unit in its last place: the sum is rounded to the nearest integer, ties to even, and its low
+            // byte is the integer's
+            const float magic = 12582912.0f;
+            const uint32_t c0 = __float_as_uint(fmaf(x[4 * w], inverse, magic)), c1 = __float_as_uint(fmaf(x[4 * w + 1], inverse, magic));
+            const uint32_t c2 = __float_as_uint(fmaf(x[4 * w + 2], inverse, magic)), c3 = __float_as_uint(fmaf(x[4 * w + 3], inverse, magic));
             word[w] = __byte_perm(__byte_perm(c0, c1, 0x0040), __byte_perm(c2, c3, 0x0040), 0x5410);
         } else {
             uint16_t lo, hi;
@@ -69,5 +73,96 @@ __device__ __forceinline__ void codes4_to_half(uint32_t word, uint32_t& lo, uint
             : "=r"(lo), "=r"(hi) : "r"(word));
     }
 }
+
+// 2^(b - 127) as packed pairs of T, in two factors: f16 scales may lie below its smallest normal number, and the product
+// of a code with the first factor is exact. Where V's byte marks a row that is not finite its codes count as zeros (the
+// row's K is NaN, which is what reaches the queries that see it).
+template <typename T>
+__device__ __forceinline__ void scaled_factors(uint32_t b, bool v, uint32_t& first, uint32_t& second);
+template <>
+__device__ __forceinline__ void scaled_factors<__nv_bfloat16>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
+    if (v && b == 255) b = 0;
+    first = (b << 7) * 0x00010001u;
+    second = 0;
+}
+template <>
+__device__ __forceinline__ void scaled_factors<__half>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
+    if (b == 255 || b == 0) {
+        first = b == 0 || v ? 0u : 0x7c007c00u;
+        second = 0x3c003c00u;
+        return;
+    }
+    const int e = int(b) - 127;
+    const int high = max(min(e, 15), -14), rest = max(min(e - high, 15), -24);
+    first = uint32_t((high + 15) << 10) * 0x00010001u;
+    // (below 2^-14 a subnormal power; scales below 2^-38 leave nothing of a code either way)
+    second = (rest >= -14 ? uint32_t((rest + 15) << 10) : 1u << (rest + 24)) * 0x00010001u;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
+template <>
+__device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+template <>
+__device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+
+// Four codes to four elements of T, exactly, unscaled.
+template <typename T, int CODE>
+__device__ __forceinline__ void codes4_to(uint32_t word, uint32_t& lo, uint32_t& hi) {
+    if constexpr (std::is_same<T, __half>::value) {
+        codes4_to_half<CODE>(word, lo, hi);
+    } else if constexpr (CODE == kCodeInt8) {
+        // bf16 has 8 significant bits: 128 + (c & 127) minus 128 (c >= 0) or 256 (c < 0), whose patterns are 0x4300 with
+        // the code's low seven bits and 0x4300 with its sign bit
+        const uint32_t a = __byte_perm(word, 0x43434343u, 0x4140), b = __byte_perm(word, 0x43434343u, 0x4342);
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a & 0xff7fff7fu), "r"(a & 0xff80ff80u));
+        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(b & 0xff7fff7fu), "r"(b & 0xff80ff80u));
+    } else {
+        // sign and the seven magnitude bits placed so that the code's exponent sits at the bottom of bf16's, times 2^120:
+        // subnormal codes come out right too (the NaN codes as +-480: a page's codes are finite, others are masked)
+        const uint32_t a = __byte_perm(word, 0u, 0x1404), b = __byte_perm(word, 0u, 0x3424);
+        lo = mul2<__nv_bfloat16>((a & 0x80008000u) | ((a >> 4) & 0x07f007f0u), 0x7b807b80u);
+        hi = mul2<__nv_bfloat16>((b & 0x80008000u) | ((b >> 4) & 0x07f007f0u), 0x7b807b80u);
+    }
+}
+
+// Values c * 2^e of four codes as packed pairs of T, rounded once; beyond f16's largest value they become infinities.
+template <typename T, int CODE>
+__device__ __forceinline__ void decode4(uint32_t word, uint32_t first, uint32_t second, uint32_t& lo, uint32_t& hi) {
+    codes4_to<T, CODE>(word, lo, hi);
+    lo = mul2<T>(lo, first);
+    hi = mul2<T>(hi, first);
+    if constexpr (std::is_same<T, __half>::value) {
+        lo = mul2<T>(lo, second);
+        hi = mul2<T>(hi, second);
+    }
+}
+
+// Infinities to the largest finite value; NaN stays.
+template <typename T>
+__device__ __forceinline__ uint32_t saturate2(uint32_t v);
+template <>
+__device__ __forceinline__ uint32_t saturate2<__half>(uint32_t v) {
+    const __half2 most = __halves2half2(__ushort_as_half(0x7bff), __ushort_as_half(0x7bff)), least = __hneg2(most);
+    const __half2 cut = __hmin2_nan(__hmax2_nan(*reinterpret_cast<__half2*>(&v), least), most);
+    return *reinterpret_cast<const uint32_t*>(&cut);
+}
+template <>
+__device__ __forceinline__ uint32_t saturate2<__nv_bfloat16>(uint32_t v) {
+    const __nv_bfloat162 most = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f), __ushort_as_bfloat16(0x7f7f)), least = __hneg2(most);
+    const __nv_bfloat162 cut = __hmin2_nan(__hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&v), least), most);
+    return *reinterpret_cast<const uint32_t*>(&cut);
+}
+// Scale bytes from which a code can leave T's range (codes are below 2^9).
+template <typename T>
+__device__ __forceinline__ constexpr uint32_t first_large_byte() { return std::is_same<T, __half>::value ? 134u : 246u; }
 
 }  // namespace kh

@@ -1,21 +1,25 @@
 // Attention over scaled 8-bit pages (scaled_kv.cuh) for wide Q tiles (prefill, up to 128 rows a task) at head_dim 128, on
 // the 5th-generation tensor cores.
 //
-//   S = Q K^T    tcgen05.mma kind::f16, M = 128 rows, N = 128 tokens; Q and K in shared memory, S in tensor memory.
+//   S = Q K^T    tcgen05.mma kind::f16, M = 128 rows, N = 64 tokens; Q and K in shared memory, S in tensor memory.
 //   O += P V     P from tensor memory (over the columns of the S it came from), V in shared memory, O in tensor memory.
 //
-// Codes become 16-bit operands of the Q/output type once per step of 128 tokens, in shared memory, with their row's
+// Codes become 16-bit operands of the Q/output type once per step of 64 tokens, in shared memory, with their row's
 // power-of-two scale already applied: int8 and E4M3 codes times 2^e are exact in bf16, and in f16 as far as its range goes
 // (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). Two Q tiles of the same
-// sequence and KV head share every converted step and take turns: while the softmax of one tile runs, the tensor cores
-// work on the other's products.
+// sequence and KV head share every converted step. A probability is rounded to the Q/output type: in bf16 that is off by
+// at most 2^-8, no more than what the cache rounds off a V element (2^-8 to 2^-7 of the row's largest).
 //
-// What bounds it: an exponential for every score (16 a cycle and SM: 1,024 cycles for a tile's 128 x 128 scores, which is
-// also about what its two products take), then instruction issue, of which the conversion takes about a third - hence
-// the two tiles per conversion.
+// Each tile has two score buffers, so that the scores of step j + 1 are computed while the softmax of step j runs and the
+// softmax warps never wait for the tensor cores in the steady state. (With one buffer of 128 tokens a tile the loop
+// softmax -> P V -> Q K^T -> softmax was a chain of 7,200 cycles a step, 3,300 of them waiting.) What bounds it then is the
+// softmax itself: an exponential for every score is 16 a cycle and SM, 1,024 cycles for 128 x 128 scores, about what the
+// two products of such a block take; and the issue slots, of which the conversion needs about as many as the softmax of
+// one tile - hence the two tiles per conversion.
 //
-// Warps: 0-3 softmax and epilogue of tile A (one thread a row), 4-7 of tile B, 8-13 conversion, 14 task decoding and
-// copies, 15 tensor-core issue (one thread). All waits are bounded (mbar_wait); no named barriers between roles.
+// Warps: 0-3 softmax and epilogue of tile A (one thread a row), 4-7 of tile B, 8-12 conversion, 13 and 15 tensor-core
+// issue (one lane, a warp for each tile), 14 task decoding and copies. All waits are bounded (mbar_wait); no named
+// barriers between roles.
 #pragma once
 
 #include "scaled_kv.cuh"
@@ -28,15 +32,17 @@ namespace kh {
 struct ScaledTc {
     static constexpr int kD = 128;
     static constexpr int kRows = 128;
-    static constexpr int kStep = 128;                            // tokens of a step
+    static constexpr int kStep = 64;                             // tokens of a step
+    static constexpr int kStages = 4;                            // steps of K and of V in shared memory
     static constexpr int kChunks = kStep / 16;                   // raw slots (16 tokens) of a step
     static constexpr int kRawSlots = 8;
     static constexpr int kRawBytes = 2 * 16 * kD;
-    static constexpr int kOperandBytes = kStep * kD * 2;         // a step's K or V, and a Q tile: two 64-element halves of
-    static constexpr int kHalfBytes = kOperandBytes / 2;         // [128 rows][128 bytes], 128-byte swizzle
-    static constexpr int kConverters = 6;
+    // a step's K or V, and a Q tile: two 64-element halves of [rows][128 bytes], 128-byte swizzle
+    static constexpr int kOperandBytes = kStep * kD * 2, kHalfBytes = kOperandBytes / 2;
+    static constexpr int kQBytes = kRows * kD * 2, kQHalfBytes = kQBytes / 2;
+    static constexpr int kConverters = 5;
     static constexpr int kThreads = 16 * 32;
-    static constexpr int kSmemBytes = 6 * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
+    static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
@@ -51,66 +57,31 @@ struct ScaledTcTask {
     uint32_t tok_begin[2], num_toks[2], kv_begin[2], kv_end[2];
 };
 
-// 2^(b - 127) as packed pairs of T, in two factors: f16 scales may lie below its smallest normal number, and the product
-// of a code with the first factor is exact. Where V's byte marks a row that is not finite its codes count as zeros (the
-// row's K is NaN, which is what reaches the queries that see it).
-template <typename T>
-__device__ __forceinline__ void scaled_factors(uint32_t b, bool v, uint32_t& first, uint32_t& second);
-template <>
-__device__ __forceinline__ void scaled_factors<__nv_bfloat16>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
-    if (v && b == 255) b = 0;
-    first = (b << 7) * 0x00010001u;
-    second = 0;
-}
-template <>
-__device__ __forceinline__ void scaled_factors<__half>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
-    if (b == 255 || b == 0) {
-        first = b == 0 || v ? 0u : 0x7c007c00u;
-        second = 0x3c003c00u;
-        return;
-    }
-    const int e = int(b) - 127;
-    const int high = max(min(e, 15), -14), rest = max(min(e - high, 15), -24);
-    first = uint32_t((high + 15) << 10) * 0x00010001u;
-    // (below 2^-14 a subnormal power; scales below 2^-38 leave nothing of a code either way)
-    second = (rest >= -14 ? uint32_t((rest + 15) << 10) : 1u << (rest + 24)) * 0x00010001u;
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b);
-template <>
-__device__ __forceinline__ uint32_t mul2<__nv_bfloat16>(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-template <>
-__device__ __forceinline__ uint32_t mul2<__half>(uint32_t a, uint32_t b) {
-    uint32_t r;
-    asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
-    return r;
-}
-
-// Four codes to four elements of T, exactly, unscaled.
-template <typename T, int CODE>
-__device__ __forceinline__ void codes4_to(uint32_t word, uint32_t& lo, uint32_t& hi) {
-    if constexpr (std::is_same<T, __half>::value) {
-        codes4_to_half<CODE>(word, lo, hi);
-    } else if constexpr (CODE == kCodeInt8) {
-        // bf16 has 8 significant bits: 128 + (c & 127) minus 128 (c >= 0) or 256 (c < 0), whose patterns are 0x4300 with
-        // the code's low seven bits and 0x4300 with its sign bit
-        const uint32_t a = __byte_perm(word, 0x43434343u, 0x4140), b = __byte_perm(word, 0x43434343u, 0x4342);
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(lo) : "r"(a & 0xff7fff7fu), "r"(a & 0xff80ff80u));
-        asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(hi) : "r"(b & 0xff7fff7fu), "r"(b & 0xff80ff80u));
-    } else {
-        lo = fp8x2_high_bytes_to_t2<__nv_bfloat16>(__byte_perm(word, 0u, 0x1404));
-        hi = fp8x2_high_bytes_to_t2<__nv_bfloat16>(__byte_perm(word, 0u, 0x3424));
-    }
-}
-
 // A wait of a whole warp: the same answer in every lane.
 __device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, const MapParams& p) {
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p));
+}
+
+// Two f32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 r;
+    asm("{ .reg .b64 a, b, c, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; mov.b64 c, {%6, %7}; fma.rn.f32x2 d, a, b, c; mov.b64 {%0, %1}, d; }"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return r;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 r;
+    asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d; }"
+        : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return r;
+}
+
+// One lane of a converged warp, the same one every time. Tensor-core instructions issued under it need no handling of
+// operands that differ between lanes, which under `lane == 0` costs each of them about a hundred cycles.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(elected));
+    return elected != 0;
 }
 
 template <typename T, int CODE>
@@ -119,30 +90,27 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     using G = ScaledTc;
     constexpr int D = G::kD;
     constexpr float kRescaleLog2 = 8.0f;  // O is rescaled only when a row maximum grows by more than 2^8
-    // bf16 probabilities carry their rounding remainder in a second product where it counts; f16 ones (11 bits) do not
-    constexpr bool kRemainder = std::is_same<T, __nv_bfloat16>::value;
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const q_tile = smem;                                  // [2]
-    uint8_t* const k_ring = smem + 2 * G::kOperandBytes;           // [2]
-    uint8_t* const v_ring = smem + 4 * G::kOperandBytes;           // [2]
-    uint8_t* const raw_ring = smem + 6 * G::kOperandBytes;         // [kRawSlots]
+    uint8_t* const k_ring = smem + 2 * G::kQBytes;                 // [kStages]
+    uint8_t* const v_ring = k_ring + G::kStages * G::kOperandBytes;
+    uint8_t* const raw_ring = v_ring + G::kStages * G::kOperandBytes;  // [kRawSlots]
     uint8_t* const raw_scales = raw_ring + G::kRawSlots * G::kRawBytes;
     ScaledTcTask* const tasks = reinterpret_cast<ScaledTcTask*>(raw_scales + G::kRawSlots * 32);  // [2]
     uint64_t* const bars = reinterpret_cast<uint64_t*>(tasks + 2);
     const uint32_t bar0 = smem_addr(bars);
     const uint32_t raw_full = bar0, raw_empty = bar0 + 64;         // [8] each
-    const uint32_t k_full = bar0 + 128, k_empty = bar0 + 144, v_full = bar0 + 160, v_empty = bar0 + 176;  // [2] each
-    const uint32_t s_full = bar0 + 192, p_full = bar0 + 208, q_full = bar0 + 224;  // [tile]
-    const uint32_t o_full = bar0 + 240, o_free = bar0 + 256, pv_done = bar0 + 272;
-    const uint32_t task_full = bar0 + 288, task_empty = bar0 + 304;  // [2]
-    const uint32_t drain = bar0 + 320;
-    constexpr int kBars = 41;
+    const uint32_t k_full = bar0 + 128, k_empty = bar0 + 160, v_full = bar0 + 192, v_empty = bar0 + 224;  // [4] each
+    const uint32_t s_full = bar0 + 256, p_full = bar0 + 288;       // [tile][buffer]
+    const uint32_t q_full = bar0 + 320, o_full = bar0 + 336, o_free = bar0 + 352, pv_done = bar0 + 368;  // [tile]
+    const uint32_t task_full = bar0 + 384, task_empty = bar0 + 400;  // [2]
+    const uint32_t drain = bar0 + 416;
+    constexpr int kBars = 53;
     volatile uint32_t* const abort_flag = reinterpret_cast<volatile uint32_t*>(bars + kBars);
     uint32_t* const tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
-    volatile uint32_t* const remainder_flag = abort_flag + 2;      // [2][4]
-    static_assert(sizeof(ScaledTcTask) * 2 + kBars * 8 + 48 <= 1024, "small shared memory");
+    static_assert(sizeof(ScaledTcTask) * 2 + kBars * 8 + 16 <= 1024, "small shared memory");
 
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
@@ -150,21 +118,23 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             mbar_init(raw_full + 8 * i, 1);
             mbar_init(raw_empty + 8 * i, 1);
         }
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             mbar_init(k_full + 8 * i, G::kChunks);
             mbar_init(v_full + 8 * i, G::kChunks);
-            mbar_init(k_empty + 8 * i, 1);
-            mbar_init(v_empty + 8 * i, 1);
+            mbar_init(k_empty + 8 * i, 2);
+            mbar_init(v_empty + 8 * i, 2);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);
+        }
+        for (int i = 0; i < 2; ++i) {
             mbar_init(q_full + 8 * i, 4);
             mbar_init(o_full + 8 * i, 1);
             mbar_init(o_free + 8 * i, 4);
             mbar_init(pv_done + 8 * i, 1);
             mbar_init(task_full + 8 * i, 1);
-            mbar_init(task_empty + 8 * i, 8 + G::kConverters + 1);
+            mbar_init(task_empty + 8 * i, 8 + G::kConverters + 2);
         }
-        mbar_init(drain, 1);
+        mbar_init(drain, 2);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -176,12 +146,11 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     __syncthreads();
     tmem_fence_after();
     const uint32_t tmem = *tmem_slot;
-    const uint32_t tmem_s = tmem, tmem_o = tmem + 256;             // + 128 * tile; P over the first 64 columns of S
+    const uint32_t tmem_s = tmem, tmem_o = tmem + 256;  // + 128 * tile (+ 64 * buffer); P over the first half of its S
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const ActiveCounts a = resolve_active(p);
 
     if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 14) {
             // ------------------------------ tasks and copies --------------------------------------------------------
             // Tasks are pairs of neighbouring templates, dealt round robin KV head by KV head, so that at any moment the
@@ -196,82 +165,143 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             const uint64_t policy = l2_evict_first_policy();
             uint32_t published = 0, issued = 0;
             bool ok = true;
-            auto decode = [&](uint32_t tmpl, uint32_t tile, ScaledTcTask& task) -> bool {
-                if (tmpl >= a.templates) return false;
-                const uint32_t range = p.templates[uint64_t(tmpl) * 3];
-                uint32_t begin, end;
-                if (p.q_ranges == nullptr) {
-                    if (range >= a.tokens) return false;
-                    begin = range;
-                    end = range + 1;
-                } else {
-                    if (range >= a.q_tiles) return false;
-                    begin = p.q_ranges[range * 2];
-                    end = p.q_ranges[range * 2 + 1];
-                    if (begin >= a.tokens || end > a.tokens || end <= begin) return false;
-                }
-                const uint32_t kv_begin = p.templates[uint64_t(tmpl) * 3 + 1], kv_end = p.templates[uint64_t(tmpl) * 3 + 2];
-                const uint32_t slot = p.req_slots[begin];
-                if (slot >= p.num_req_slots ||
-                    (kv_end > kv_begin && (uint64_t(kv_end) + p.tokens_per_page - 1) / p.tokens_per_page > p.pages_per_request_layer)) {
-                    if (lane == 0) atomicOr(p.status, kStatusMetadataOutOfRange);
-                    return false;
-                }
-                task.tmpl[tile] = tmpl;
-                task.tok_begin[tile] = begin;
-                task.num_toks[tile] = min(end - begin, p.max_q_tokens);
-                // what some row of the tile sees
-                uint32_t lo = 0xffffffffu, hi = 0;
-                for (uint32_t tok = lane; tok < task.num_toks[tile]; tok += 32) {
-                    uint32_t l, h;
-                    scaled_visible(p, begin, tok, kv_begin, kv_end, l, h);
-                    if (h > l) {
-                        lo = min(lo, l);
-                        hi = max(hi, h);
+            // Two neighbouring templates at once, a half warp each: is there a tile to work on, and for which request.
+            auto decode = [&](uint32_t tmpl0, ScaledTcTask& task, uint32_t& slot0, uint32_t& slot1) -> uint32_t {
+                const uint32_t tile = lane >> 4, sub = lane & 15, tmpl = tmpl0 + tile;
+                uint32_t there = 0, begin = 0, num = 0, slot = 0, lo = 0xffffffffu, hi = 0;
+                if (tmpl < a.templates && (tile == 0 || stride == 2)) {
+                    const uint32_t range = p.templates[uint64_t(tmpl) * 3];
+                    const uint32_t kv_begin = p.templates[uint64_t(tmpl) * 3 + 1], kv_end = p.templates[uint64_t(tmpl) * 3 + 2];
+                    uint32_t end = 0;
+                    if (p.q_ranges == nullptr) {
+                        there = range < a.tokens;
+                        begin = range;
+                        end = range + 1;
+                    } else if (range < a.q_tiles) {
+                        begin = p.q_ranges[range * 2];
+                        end = p.q_ranges[range * 2 + 1];
+                        there = begin < a.tokens && end <= a.tokens && end > begin;
+                    }
+                    if (there) {
+                        num = min(end - begin, p.max_q_tokens);
+                        slot = p.req_slots[begin];
+                        // what some row of the tile sees
+                        for (uint32_t tok = sub; tok < num; tok += 16) {
+                            uint32_t l, h;
+                            scaled_visible(p, begin, tok, kv_begin, kv_end, l, h);
+                            if (h > l) {
+                                lo = min(lo, l);
+                                hi = max(hi, h);
+                            }
+                        }
+                        if (slot >= p.num_req_slots || (kv_end > kv_begin && (uint64_t(kv_end) + p.tokens_per_page - 1) / p.tokens_per_page >
+                                                                                 p.pages_per_request_layer)) {
+                            if (sub == 0) atomicOr(p.status, kStatusMetadataOutOfRange);  // the task is dropped, as in decode_task
+                            there = 0;
+                        }
                     }
                 }
-                lo = __reduce_min_sync(0xffffffffu, lo);
-                hi = __reduce_max_sync(0xffffffffu, hi);
-                task.kv_begin[tile] = hi > lo ? lo : 0;
-                task.kv_end[tile] = hi > lo ? hi : 0;
-                if (tile == 0) task.req_slot = slot;
-                return tile == 0 || slot == task.req_slot;
+#pragma unroll
+                for (int d = 8; d >= 1; d >>= 1) {
+                    lo = min(lo, __shfl_xor_sync(0xffffffffu, lo, d));
+                    hi = max(hi, __shfl_xor_sync(0xffffffffu, hi, d));
+                }
+                if (hi <= lo) lo = hi = 0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    task.tmpl[i] = tmpl0 + i;
+                    task.tok_begin[i] = __shfl_sync(0xffffffffu, begin, 16 * i);
+                    task.num_toks[i] = __shfl_sync(0xffffffffu, num, 16 * i);
+                    task.kv_begin[i] = __shfl_sync(0xffffffffu, lo, 16 * i);
+                    task.kv_end[i] = __shfl_sync(0xffffffffu, hi, 16 * i);
+                }
+                slot0 = __shfl_sync(0xffffffffu, slot, 0);
+                slot1 = __shfl_sync(0xffffffffu, slot, 16);
+                return __shfl_sync(0xffffffffu, there, 0) | (__shfl_sync(0xffffffffu, there, 16) << 1);
             };
-            // publishes the task and streams its raw slots
-            auto stream = [&](ScaledTcTask& task) {
-                if (!ok) return;
+            // This CTA's next task, in order. Every other round of the deal runs backwards: tasks next to one another
+            // differ little in length.
+            uint64_t round = 0;
+            bool second_left = false;  // the second tile of the last pair is a task of its own
+            uint32_t second_slot = 0;
+            ScaledTcTask task{};
+            auto next_task = [&]() {
+                if (second_left) {
+                    second_left = false;
+                    task.tmpl[0] = task.tmpl[1];
+                    task.tok_begin[0] = task.tok_begin[1];
+                    task.num_toks[0] = task.num_toks[1];
+                    task.kv_begin[0] = task.kv_begin[1];
+                    task.kv_end[0] = task.kv_end[1];
+                    task.req_slot = second_slot;
+                    task.active_b = 0;
+                } else {
+                    uint32_t found = 0;
+                    while (found == 0) {
+                        const uint64_t index = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+                        if (round * gridDim.x >= total) {
+                            task.done = 1;
+                            task.steps = 0;
+                            return;
+                        }
+                        ++round;
+                        if (index >= total) continue;
+                        const uint32_t cell = uint32_t(index / pairs), pair = pairs - 1 - uint32_t(index % pairs);
+                        task.kv_head = cell / p.head_ranges;
+                        const uint32_t skipped = (cell % p.head_ranges) * p.heads_per_task;
+                        task.head_begin = task.kv_head * p.group + skipped;
+                        task.num_heads = min(p.heads_per_task, p.group - skipped);
+                        uint32_t slot0, slot1;
+                        found = decode(stride * pair, task, slot0, slot1);
+                        second_slot = slot1;
+                        task.req_slot = slot0;
+                        // two tiles of one request that begin together; else one after the other
+                        task.active_b = found == 3 && slot0 == slot1 && task.kv_begin[0] == task.kv_begin[1] ? 1 : 0;
+                        second_left = found == 3 && task.active_b == 0;
+                        if (found == 2) {
+                            task.tmpl[0] = task.tmpl[1];
+                            task.tok_begin[0] = task.tok_begin[1];
+                            task.num_toks[0] = task.num_toks[1];
+                            task.kv_begin[0] = task.kv_begin[1];
+                            task.kv_end[0] = task.kv_end[1];
+                            task.req_slot = slot1;
+                        }
+                    }
+                }
                 task.begin = task.kv_begin[0];
-                task.end = task.kv_end[0];
-                if (task.active_b) task.end = max(task.end, task.kv_end[1]);  // (tiles together begin together)
+                task.end = task.active_b ? max(task.kv_end[0], task.kv_end[1]) : task.kv_end[0];  // (they begin together)
                 task.first = task.begin / 16 * 16;
                 task.steps = task.end > task.first ? (task.end - task.first + G::kStep - 1) / G::kStep : 0;
+            };
+            next_task();
+            while (ok) {
                 const uint32_t ts = published & 1;
-                if (!mbar_wait_warp(task_empty + 8 * ts, ((published >> 1) & 1) ^ 1, abort_flag, p)) {
-                    ok = false;
-                    return;
-                }
+                ok = mbar_wait_warp(task_empty + 8 * ts, ((published >> 1) & 1) ^ 1, abort_flag, p);
+                if (!ok) break;
                 if (lane == 0) {
                     tasks[ts] = task;
                     mbar_arrive(task_full + 8 * ts);
                 }
                 ++published;
-                if (task.done) return;
+                if (task.done) break;
+                // what streaming needs; the next task is decoded on the way, once the ring is full
+                const uint32_t begin = task.begin, end = task.end, first = task.first, kv_head = task.kv_head;
                 const uint64_t table = (uint64_t(task.req_slot) * p.num_gqa_layers + p.layer_index) * p.pages_per_request_layer;
-                const uint32_t slots = task.end > task.first ? (task.end - task.first + 15) / 16 : 0;
+                const uint64_t scales = uint64_t((p.num_kv_heads * 2) << page_shift) * D + ((kv_head * 2) << page_shift);
+                const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
                 uint32_t page0 = 0, page1 = 0;
-                for (uint32_t x = 0; x < slots; ++x) {
-                    if ((x & 31) == 0) {
-                        const uint32_t token = task.first + (x + lane) * 16;
-                        if (x + lane < slots) {
-                            // (the first half may lie before everything that is visible, the second behind it)
-                            const bool low = token + 8 > task.begin || token + 8 >= task.end;
-                            page0 = p.page_ids[table + ((low ? token : token + 8) >> page_shift)];
-                            page1 = page_shift == 3 && low && token + 8 < task.end ? p.page_ids[table + ((token + 8) >> page_shift)] : page0;
-                            if (page0 >= p.pool_pages || page1 >= p.pool_pages) {
-                                atomicOr(p.status, kStatusPageOutOfPool);  // nothing outside the pool is read
-                                if (page0 >= p.pool_pages) page0 = 0;
-                                if (page1 >= p.pool_pages) page1 = 0;
-                            }
+                if (slots == 0) next_task();
+                for (uint32_t x = 0; x < slots && ok; ++x) {
+                    if ((x & 31) == 0 && x + lane < slots) {
+                        const uint32_t token = first + (x + lane) * 16;
+                        // (the first half may lie before everything that is visible, the second behind it)
+                        const bool low = token + 8 > begin || token + 8 >= end;
+                        page0 = p.page_ids[table + ((low ? token : token + 8) >> page_shift)];
+                        page1 = page_shift == 3 && low && token + 8 < end ? p.page_ids[table + ((token + 8) >> page_shift)] : page0;
+                        if (page0 >= p.pool_pages || page1 >= p.pool_pages) {
+                            atomicOr(p.status, kStatusPageOutOfPool);  // nothing outside the pool is read
+                            if (page0 >= p.pool_pages) page0 = 0;
+                            if (page1 >= p.pool_pages) page1 = 0;
                         }
                     }
                     const uint32_t first_page = __shfl_sync(0xffffffffu, page0, int(x & 31)), second_page = __shfl_sync(0xffffffffu, page1, int(x & 31));
@@ -281,12 +311,10 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         if (ok) {
                             const uint32_t bar = raw_full + 8 * slot, dst = smem_addr(raw_ring) + slot * G::kRawBytes;
                             const uint32_t sdst = smem_addr(raw_scales) + slot * 32;
-                            const uint32_t row = (task.kv_head << page_shift) + ((task.first + x * 16) & (p.tokens_per_page - 1));
                             mbar_arrive_expect_tx(bar, G::kRawBytes + 32);
-                            const uint64_t scales = uint64_t((p.num_kv_heads * 2) << page_shift) * D + ((task.kv_head * 2) << page_shift);
-                            tma_load_5d(dst, &kv_map, int32_t(row), int32_t(first_page), bar, policy);
+                            tma_load_5d(dst, &kv_map, int32_t(kv_head << page_shift), int32_t(first_page), bar, policy);
                             if (page_shift == 3) {
-                                tma_load_5d(dst + G::kRawBytes / 2, &kv_map, int32_t(row), int32_t(second_page), bar, policy);
+                                tma_load_5d(dst + G::kRawBytes / 2, &kv_map, int32_t(kv_head << page_shift), int32_t(second_page), bar, policy);
                                 bulk_load(sdst, p.kv_pages + uint64_t(first_page) * p.page_bytes + scales, 16, bar);
                                 bulk_load(sdst + 16, p.kv_pages + uint64_t(second_page) * p.page_bytes + scales, 16, bar);
                             } else {
@@ -296,29 +324,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     }
                     ++issued;
                     ok = __all_sync(0xffffffffu, ok);
-                    if (!ok) return;
-                }
-            };
-            for (uint64_t index = blockIdx.x; index < total && ok; index += gridDim.x) {
-                const uint32_t cell = uint32_t(index / pairs), pair = pairs - 1 - uint32_t(index % pairs);
-                ScaledTcTask task{};
-                task.kv_head = cell / p.head_ranges;
-                const uint32_t skipped = (cell % p.head_ranges) * p.heads_per_task;
-                task.head_begin = task.kv_head * p.group + skipped;
-                task.num_heads = min(p.heads_per_task, p.group - skipped);
-                // two tiles of one request that begin together; else one after the other
-                const bool first = decode(stride * pair, 0, task);
-                const bool together = first && stride == 2 && decode(2 * pair + 1, 1, task) && task.kv_begin[0] == task.kv_begin[1];
-                task.active_b = together ? 1 : 0;
-                if (first) stream(task);
-                if (!together && stride == 2) {
-                    task.active_b = 0;
-                    if (decode(2 * pair + 1, 0, task)) stream(task);
+                    if (x == min(slots, uint32_t(G::kRawSlots)) - 1) next_task();
                 }
             }
-            ScaledTcTask last{};
-            last.done = 1;
-            stream(last);
             if (*abort_flag && lane == 0) {
                 // copies already issued may still be landing
                 for (uint32_t back = 0; back < uint32_t(G::kRawSlots) && back < issued; ++back) {
@@ -328,94 +336,102 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     }
                 }
             }
-        } else if (warp == 15) {
-            // ------------------------------ tensor-core issue (one thread) -------------------------------------------
-            if (lane == 0) {
-                constexpr uint32_t kFormat = umma_format<T>();
-                constexpr uint32_t idesc_qk = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 3) << 17) | ((128u >> 4) << 24);
-                constexpr uint32_t idesc_pv = idesc_qk | (1u << 16);  // B (V) is stored with the head dimension innermost
-                const uint64_t k_desc0 = umma_smem_desc(0, 16, 1024);
-                const uint64_t v_desc0 = umma_smem_desc(0, G::kHalfBytes, 1024);
-                const uint32_t q_addr = smem_addr(q_tile), k_addr = smem_addr(k_ring), v_addr = smem_addr(v_ring);
-                uint32_t k_step = 0, v_step = 0;        // running step numbers of the rings
-                uint32_t p_count[2] = {0, 0}, pv_count[2] = {0, 0}, q_count[2] = {0, 0}, o_count[2] = {0, 0};
-                bool ok = true;
-                auto qk = [&](uint32_t tile) {
-                    tmem_fence_after();
-                    const uint64_t q = k_desc0 + uint64_t((q_addr + tile * G::kOperandBytes) >> 4);
-                    const uint64_t k = k_desc0 + uint64_t((k_addr + (k_step & 1) * G::kOperandBytes) >> 4);
+        } else if (warp >= 8 + G::kConverters) {
+            // ------------------------------ tensor-core issue: a warp for each tile, one lane issues ------------------
+            const uint32_t tile = warp == 15 ? 1 : 0;
+            constexpr uint32_t kFormat = umma_format<T>();
+            constexpr uint32_t idesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
+            constexpr uint32_t idesc_qk = idesc | ((uint32_t(G::kStep) >> 3) << 17);
+            constexpr uint32_t idesc_pv = idesc | ((uint32_t(D) >> 3) << 17) | (1u << 16);  // V: head dimension innermost
+            const uint64_t k_desc0 = umma_smem_desc(0, 16, 1024);
+            const uint64_t v_desc0 = umma_smem_desc(0, G::kHalfBytes, 1024);
+            const uint64_t q_desc = k_desc0 + uint64_t((smem_addr(q_tile) + tile * G::kQBytes) >> 4);
+            const uint32_t k_addr = smem_addr(k_ring), v_addr = smem_addr(v_ring);
+            const uint32_t scores = tmem_s + 128 * tile, out = tmem_o + 128 * tile;
+            uint32_t step = 0;                              // running step number of the K and V rings
+            uint32_t mine = 0;                              // running step number of this tile
+            uint32_t done_tasks = 0;                        // of this tile
+            bool ok = true;
+            auto stage_wait = [&](uint32_t bar, uint32_t number) {
+                return mbar_wait_warp(bar + 8 * (number % G::kStages), (number / G::kStages) & 1, abort_flag, p);
+            };
+            // scores of step `ahead` steps on, into their buffer
+            auto issue_scores = [&](uint32_t ahead) {
+                tmem_fence_after();
+                const uint32_t stage = (step + ahead) % G::kStages, buffer = (mine + ahead) & 1;
+                const uint64_t k = k_desc0 + uint64_t((k_addr + stage * G::kOperandBytes) >> 4);
+                if (elect_one()) {
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk) {
-                        const uint64_t at = uint64_t(((kk / 4) * G::kHalfBytes + (kk % 4) * 32) >> 4);
-                        umma_ss(tmem_s + 128 * tile, q + at, k + at, idesc_qk, kk > 0 ? 1u : 0u);
+                        umma_ss(scores + 64 * buffer, q_desc + uint64_t(((kk / 4) * G::kQHalfBytes + (kk % 4) * 32) >> 4),
+                                k + uint64_t(((kk / 4) * G::kHalfBytes + (kk % 4) * 32) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
                     }
-                    umma_commit(s_full + 8 * tile);
-                };
-                for (uint32_t taken = 0; ok; ++taken) {
-                    const uint32_t ts = taken & 1;
-                    if (!mbar_wait(task_full + 8 * ts, (taken >> 1) & 1, abort_flag, p)) break;
-                    if (tasks[ts].done) break;
-                    const uint32_t steps = tasks[ts].steps, tiles = 1 + tasks[ts].active_b;
-                    mbar_arrive(task_empty + 8 * ts);
-                    for (uint32_t j = 0; j <= steps && ok && steps > 0; ++j) {
-                        // products of step j - 1 with V, then scores of step j; tile by tile
-                        if (j < steps) ok = mbar_wait(k_full + 8 * (k_step & 1), (k_step >> 1) & 1, abort_flag, p);
-                        for (uint32_t tile = 0; tile < tiles && ok; ++tile) {
-                            if (j > 0) {
-                                ok = mbar_wait(p_full + 8 * tile, p_count[tile] & 1, abort_flag, p);
-                                ++p_count[tile];
-                                if (ok && tile == 0) ok = mbar_wait(v_full + 8 * (v_step & 1), (v_step >> 1) & 1, abort_flag, p);
-                                if (ok && j == 1) {
-                                    // the tile's first product overwrites O: its last epilogue must have read it
-                                    ok = mbar_wait(o_free + 8 * tile, (o_count[tile] & 1) ^ 1, abort_flag, p);
-                                    ++o_count[tile];
-                                }
-                                if (!ok) break;
-                                tmem_fence_after();
-                                const bool with_remainder = kRemainder && (remainder_flag[4 * tile] | remainder_flag[4 * tile + 1] |
-                                                                           remainder_flag[4 * tile + 2] | remainder_flag[4 * tile + 3]) != 0u;
-                                const uint64_t v = v_desc0 + uint64_t((v_addr + (v_step & 1) * G::kOperandBytes) >> 4);
-                                const uint32_t probabilities = tmem_s + 128 * tile;
-#pragma unroll
-                                for (int i = 0; i < G::kStep / 16; ++i) {
-                                    umma_ts(tmem_o + 128 * tile, probabilities + 8 * i, v + uint64_t((i * 2048) >> 4), idesc_pv, j > 1 || i > 0 ? 1u : 0u);
-                                }
-                                if (with_remainder) {
-#pragma unroll
-                                    for (int i = 0; i < G::kStep / 16; ++i) {
-                                        umma_ts(tmem_o + 128 * tile, probabilities + 64 + 8 * i, v + uint64_t((i * 2048) >> 4), idesc_pv, 1u);
-                                    }
-                                }
-                                umma_commit(pv_done + 8 * tile);
-                                if (tile + 1 == tiles) umma_commit(v_empty + 8 * (v_step & 1));
-                                if (j == steps) umma_commit(o_full + 8 * tile);
-                            }
-                            if (j < steps) {
-                                if (j == 0) {
-                                    ok = mbar_wait(q_full + 8 * tile, q_count[tile] & 1, abort_flag, p);
-                                    ++q_count[tile];
-                                } else {
-                                    // the scores go where the probabilities of the product before lie
-                                    ok = mbar_wait(pv_done + 8 * tile, pv_count[tile] & 1, abort_flag, p);
-                                }
-                                if (!ok) break;
-                                qk(tile);
-                            }
-                            if (j > 0) ++pv_count[tile];
+                    umma_commit(s_full + 8 * (2 * tile + buffer));
+                    umma_commit(k_empty + 8 * stage);
+                }
+                __syncwarp();
+            };
+            for (uint32_t taken = 0; ok; ++taken) {
+                const uint32_t ts = taken & 1;
+                if (!mbar_wait_warp(task_full + 8 * ts, (taken >> 1) & 1, abort_flag, p)) break;
+                if (tasks[ts].done) break;
+                const uint32_t steps = tasks[ts].steps;
+                const bool here = tile == 0 || tasks[ts].active_b != 0;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(task_empty + 8 * ts);
+                if (!here) {
+                    // the steps pass by: this warp's arrivals on their slots
+                    for (uint32_t j = 0; j < steps && ok; ++j, ++step) {
+                        ok = stage_wait(k_full, step) && stage_wait(v_full, step);
+                        if (ok && lane == 0) {
+                            mbar_arrive(k_empty + 8 * (step % G::kStages));
+                            mbar_arrive(v_empty + 8 * (step % G::kStages));
                         }
-                        if (!ok) break;
-                        if (j < steps) {
-                            umma_commit(k_empty + 8 * (k_step & 1));
-                            ++k_step;
-                        }
-                        if (j > 0) ++v_step;
                     }
+                    continue;
                 }
-                // nothing issued here may still be running when tensor memory is freed (bounded, also on the abort path)
-                umma_commit(drain);
-                for (uint32_t i = 0; i < p.wait_limit; ++i) {
-                    if (mbar_try_wait(drain, 0)) break;
+                if (steps == 0) continue;
+                ok = mbar_wait_warp(q_full + 8 * tile, done_tasks & 1, abort_flag, p) && stage_wait(k_full, step);
+                if (!ok) break;
+                // (both buffers are free: every product of the task before has been waited for)
+                issue_scores(0);
+                if (steps > 1) {
+                    ok = stage_wait(k_full, step + 1);
+                    if (!ok) break;
+                    issue_scores(1);
                 }
+                for (uint32_t j = 0; j < steps && ok; ++j, ++step, ++mine) {
+                    // step j: the product with V, then the scores of step j + 2, which go where its probabilities lie
+                    const uint32_t buffer = mine & 1;
+                    ok = mbar_wait_warp(p_full + 8 * (2 * tile + buffer), (mine >> 1) & 1, abort_flag, p) && stage_wait(v_full, step);
+                    // the tile's first product overwrites O: its last epilogue must have read it
+                    if (ok && j == 0) ok = mbar_wait_warp(o_free + 8 * tile, (done_tasks & 1) ^ 1, abort_flag, p);
+                    if (!ok) break;
+                    tmem_fence_after();
+                    const uint32_t stage = step % G::kStages;
+                    const uint64_t v = v_desc0 + uint64_t((v_addr + stage * G::kOperandBytes) >> 4);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < G::kStep / 16; ++i) {
+                            umma_ts(out, scores + 64 * buffer + 8 * i, v + uint64_t((i * 2048) >> 4), idesc_pv, j > 0 || i > 0 ? 1u : 0u);
+                        }
+                        umma_commit(pv_done + 8 * tile);
+                        umma_commit(v_empty + 8 * stage);
+                        if (j + 1 == steps) umma_commit(o_full + 8 * tile);
+                    }
+                    __syncwarp();
+                    if (j + 2 < steps) ok = stage_wait(k_full, step + 2);
+                    ok = ok && mbar_wait_warp(pv_done + 8 * tile, mine & 1, abort_flag, p);
+                    if (!ok) break;
+                    if (j + 2 < steps) issue_scores(2);
+                }
+                ++done_tasks;
+            }
+            // nothing issued here may still be running when tensor memory is freed (bounded, also on the abort path)
+            if (elect_one()) umma_commit(drain);
+            __syncwarp();
+            for (uint32_t i = 0; i < p.wait_limit; ++i) {
+                if (mbar_try_wait(drain, 0)) break;
             }
         } else {
             // ------------------------------ conversion ---------------------------------------------------------------
@@ -424,7 +440,12 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             // stores, touch every bank once (128-byte swizzle on both sides).
             const uint32_t sub = (lane >> 2) & 1, cc = lane & 3, row_pair = lane >> 4, flip = (lane >> 3) & 1;
             const uint32_t row4 = 2 * row_pair + (sub ^ flip), piece = 4 * sub + cc;
+            // Rows 4 i + row4, i < 4. A copy holds [K/V][16 rows], or two of [K/V][8 rows] (8-token pages); scale bytes alike.
             const bool short_pages = p.tokens_per_page == 8;
+            const uint32_t in_lane = row4 * 128 + ((piece ^ row4) << 4);
+            const uint32_t out_lane = sub * G::kHalfBytes + row4 * 128 + (((2 * cc) ^ row4) << 4);
+            const uint32_t plane_stride = short_pages ? 1024 : 2048, half_stride = short_pages ? 2048 : 1024;
+            const uint32_t scale_plane = short_pages ? 8 : 16, scale_half = short_pages ? 16 : 8;
             uint32_t step = 0, raw = 0, chunk_number = 0;  // running numbers
             bool ok = true;
             for (uint32_t taken = 0; ok; ++taken) {
@@ -435,89 +456,81 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(task_empty + 8 * ts);
                 const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
-                for (uint32_t j = 0; j < steps && ok; ++j, ++step) {
-                    const uint32_t stage = step & 1, phase = (step >> 1) & 1;
-                    for (uint32_t c = 0; c < uint32_t(G::kChunks); ++c, ++chunk_number) {
-                        const uint32_t x = j * G::kChunks + c;
-                        const uint32_t raw_number = raw + x;
-                        if (chunk_number % G::kConverters != warp - 8) continue;
-                        const bool there = x < slots;
-                        const uint32_t slot = raw_number % G::kRawSlots;
-                        if (there) ok = mbar_wait_warp(raw_full + 8 * slot, (raw_number / G::kRawSlots) & 1, abort_flag, p);
-                        const uint8_t* const source = raw_ring + slot * G::kRawBytes;
-                        const uint8_t* const scales = raw_scales + slot * 32;
+                for (uint32_t x = 0; x < steps * G::kChunks && ok; ++x, ++chunk_number) {
+                    if (chunk_number % G::kConverters != warp - 8) continue;
+                    const uint32_t number = step + x / G::kChunks, stage = number % G::kStages, phase = (number / G::kStages) & 1;
+                    const uint32_t raw_number = raw + x, slot = raw_number % G::kRawSlots;
+                    const bool there = x < slots;
+                    if (there) ok = mbar_wait_warp(raw_full + 8 * slot, (raw_number / G::kRawSlots) & 1, abort_flag, p);
+                    const uint8_t* const source = raw_ring + slot * G::kRawBytes;
+                    const uint8_t* const scales = raw_scales + slot * 32 + row4;
+                    const uint32_t token = first + x * 16;
+                    const bool whole = there && token >= begin && token + 16 <= end;
 #pragma unroll
-                        for (int plane = 0; plane < 2; ++plane) {
-                            ok = ok && mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
-                            if (!ok) break;
-                            uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (piece >> 2) * G::kHalfBytes;
-                            uint4 words[4];
-                            uint32_t one[4], two[4];
+                    for (int plane = 0; plane < 2; ++plane) {
+                        ok = ok && mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
+                        if (!ok) break;
+                        uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
+                        uint4 words[4];
+                        uint32_t b[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t at = plane * plane_stride + (i >> 1) * half_stride + (i & 1) * 512;
+                            words[i] = *reinterpret_cast<const uint4*>(source + at + (in_lane ^ ((i & 1) * 64)));
+                            b[i] = scales[plane * scale_plane + (i >> 1) * scale_half + (i & 1) * 4];
+                        }
+                        if (!whole) {  // rows that nothing sees may hold anything
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t t = token + 4 * i + row4;
+                                if (!there || t < begin || t >= end) {
+                                    words[i] = make_uint4(0, 0, 0, 0);
+                                    b[i] = 0;
+                                }
+                            }
+                        }
+                        bool saturate = false;
+                        if constexpr (std::is_same<T, __half>::value) {
                             bool large = false;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t row = 4 * i + row4;
-                                words[i] = make_uint4(0, 0, 0, 0);
-                                uint32_t b = 0;
-                                const uint32_t token = first + x * 16 + row;
-                                if (there && token >= begin && token < end) {
-                                    // (a copy holds [K/V][16 rows], or two of [K/V][8 rows]; scale bytes alike)
-                                    const uint32_t at = short_pages ? (row >> 3) * (G::kRawBytes / 2) + plane * 1024 + (row & 7) * 128
-                                                                    : uint32_t(plane) * 2048 + row * 128;
-                                    words[i] = *reinterpret_cast<const uint4*>(source + at + ((piece ^ (row & 7)) << 4));
-                                    b = scales[short_pages ? (row >> 3) * 16 + plane * 8 + (row & 7) : plane * 16 + row];
-                                }
-                                scaled_factors<T>(b, plane == 1, one[i], two[i]);
-                                large = large || (b >= 134 && b < 255);  // 2^7: E4M3 codes reach 448
-                            }
-                            const bool saturate = std::is_same<T, __half>::value && __any_sync(0xffffffffu, large);
-#pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t row = 4 * i + row4;
-                                const uint32_t raw_words[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
-                                uint32_t r[8];
-#pragma unroll
-                                for (int w = 0; w < 4; ++w) {
-                                    codes4_to<T, CODE>(raw_words[w], r[2 * w], r[2 * w + 1]);
-#pragma unroll
-                                    for (int e = 0; e < 2; ++e) {
-                                        uint32_t& v = r[2 * w + e];
-                                        v = mul2<T>(v, one[i]);
-                                        if constexpr (std::is_same<T, __half>::value) {
-                                            v = mul2<T>(v, two[i]);
-                                            if (saturate) {
-                                                // (2^16 is the one value past f16's largest that a code of an f16 row stands for; NaN stays)
-                                                const __half2 most = __floats2half2_rn(65504.0f, 65504.0f), least = __floats2half2_rn(-65504.0f, -65504.0f);
-                                                const __half2 cut = __hmin2_nan(__hmax2_nan(*reinterpret_cast<__half2*>(&v), least), most);
-                                                v = *reinterpret_cast<const uint32_t*>(&cut);
-                                            }
-                                        }
-                                    }
-                                }
-                                const uint32_t out_row = c * 16 + row;
-                                const uint32_t position = (2 * cc) ^ (out_row & 7);
-                                *reinterpret_cast<uint4*>(out + out_row * 128 + position * 16) = make_uint4(r[0], r[1], r[2], r[3]);
-                                *reinterpret_cast<uint4*>(out + out_row * 128 + (position ^ 1) * 16) = make_uint4(r[4], r[5], r[6], r[7]);
-                            }
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                            if (lane == 0) mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
+                            for (int i = 0; i < 4; ++i) large = large || (b[i] >= first_large_byte<T>() && b[i] < 255);
+                            saturate = __any_sync(0xffffffffu, large);
                         }
-                        if (!ok) break;
-                        if (there && lane == 0) mbar_arrive(raw_empty + 8 * slot);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t one, two;
+                            scaled_factors<T>(b[i], plane == 1, one, two);
+                            const uint32_t raw_words[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
+                            uint32_t r[8];
+#pragma unroll
+                            for (int w = 0; w < 4; ++w) decode4<T, CODE>(raw_words[w], one, two, r[2 * w], r[2 * w + 1]);
+                            if (std::is_same<T, __half>::value && saturate) {
+                                // (2^16 is the one value past f16's largest that a code of an f16 row stands for)
+#pragma unroll
+                                for (int w = 0; w < 8; ++w) r[w] = saturate2<T>(r[w]);
+                            }
+                            // rows 4-7 of an eight-row swizzle period: position bit 2 flips
+                            uint8_t* const row = out + i * 512;
+                            *reinterpret_cast<uint4*>(row + (out_lane ^ ((i & 1) * 64))) = make_uint4(r[0], r[1], r[2], r[3]);
+                            *reinterpret_cast<uint4*>(row + (out_lane ^ ((i & 1) * 64) ^ 16)) = make_uint4(r[4], r[5], r[6], r[7]);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
                     }
+                    if (ok && there && lane == 0) mbar_arrive(raw_empty + 8 * slot);
                 }
+                step += steps;
                 raw += slots;
             }
         }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
         // ------------------------------ softmax and epilogue of one tile: a thread per row ----------------------------
         const uint32_t tile = warp / 4, quad = warp % 4;
         const uint32_t row = quad * 32 + lane;
         const uint32_t lane_base = (quad * 32) << 16;
-        const uint32_t s_at = tmem_s + 128 * tile + lane_base, o_at = tmem_o + 128 * tile + lane_base;
-        uint32_t s_count = 0, o_count = 0;
+        const uint32_t o_at = tmem_o + 128 * tile + lane_base;
+        uint32_t mine = 0, done_tasks = 0;  // running numbers of this tile: steps, tasks
         bool ok = true;
         for (uint32_t taken = 0; ok; ++taken) {
             const uint32_t ts = taken & 1;
@@ -539,22 +552,23 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             if (lane == 0) mbar_arrive(task_empty + 8 * ts);  // the descriptor has been read
             if (!here) continue;
             if (steps > 0) {
-                // the row's Q into its tile (the tile's last product with the Q before has completed: its scores were read)
-                uint8_t* const dst = q_tile + tile * G::kOperandBytes + row * 128;
+                // the row's Q into its tile (the scores of the tile's last task have all been read: nothing uses it any more)
+                uint8_t* const dst = q_tile + tile * G::kQBytes + row * 128;
                 const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + q_row * D);
 #pragma unroll
                 for (int c = 0; c < 16; ++c) {
                     const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(dst + (c / 8) * G::kHalfBytes + (((c % 8) ^ (row & 7)) << 4)) = v;
+                    *reinterpret_cast<uint4*>(dst + (c / 8) * G::kQHalfBytes + (((c % 8) ^ (row & 7)) << 4)) = v;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive(q_full + 8 * tile);
             }
             float m = -INFINITY, l = 0.0f;  // m: raw dot products
-            for (uint32_t j = 0; j < steps; ++j) {
-                ok = mbar_wait_warp(s_full + 8 * tile, s_count & 1, abort_flag, p);
-                ++s_count;
+            for (uint32_t j = 0; j < steps; ++j, ++mine) {
+                const uint32_t buffer = mine & 1;
+                const uint32_t s_at = tmem_s + 128 * tile + 64 * buffer + lane_base;
+                ok = mbar_wait_warp(s_full + 8 * (2 * tile + buffer), (mine >> 1) & 1, abort_flag, p);
                 if (!ok) break;
                 tmem_fence_after();
                 uint32_t s[G::kStep];
@@ -562,17 +576,21 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 for (int c = 0; c < G::kStep; c += 32) tmem_ld32(*reinterpret_cast<uint32_t(*)[32]>(&s[c]), s_at + c);
                 tmem_ld_wait();
                 const uint32_t tok = first + j * G::kStep;
-                float top = -INFINITY;
                 if (__any_sync(0xffffffffu, tok < lo || tok + G::kStep > hi)) {
 #pragma unroll
                     for (int c = 0; c < G::kStep; ++c) {
                         if (!(tok + c >= lo && tok + c < hi)) s[c] = 0xff800000u;  // -inf
-                        top = fmaxf(top, __uint_as_float(s[c]));
                     }
-                } else {
-#pragma unroll
-                    for (int c = 0; c < G::kStep; ++c) top = fmaxf(top, __uint_as_float(s[c]));
                 }
+                float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int c = 0; c < G::kStep; c += 8) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        tops[i] = fmaxf(fmaxf(tops[i], __uint_as_float(s[c + 2 * i])), __uint_as_float(s[c + 2 * i + 1]));
+                    }
+                }
+                const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 // lazy maximum: moved (with the sum and O) only when the step exceeds it by more than 2^8
                 const bool grow = top > -INFINITY && (m == -INFINITY || (top - m) * p.scale_log2e > kRescaleLog2);
                 if (__any_sync(0xffffffffu, grow)) {
@@ -581,65 +599,52 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         l *= keep;
                         m = top;
                     }
-                    if (j > 0) {  // (the commit behind the scores covers the products before them: O is at rest)
+                    if (j > 0) {
+                        // O is at rest once the product of the step before has completed
+                        ok = mbar_wait_warp(pv_done + 8 * tile, (mine - 1) & 1, abort_flag, p);
+                        if (!ok) break;
+                        tmem_fence_after();
 #pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            tmem_ld32(o, o_at + c);
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(o, o_at + c);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                            tmem_st32(o_at + c, o);
+                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                            tmem_st16(o_at + c, o);
                         }
                         tmem_st_wait();
                     }
                 }
                 const float shift = m == -INFINITY ? 0.0f : -m * p.scale_log2e;
-                // The remainder of a bf16 probability is 2^-9 of it at most. Where the row's sum so far is 64 times the
-                // step's largest probability, dropping the step's remainders changes the output by less than 2^-9 / 8 of a
-                // V element; the product is left out when that holds for all rows of the tile.
-                bool remainder = false;
-                if constexpr (kRemainder) {
-                    const float most = top == -INFINITY ? 0.0f : fast_exp2(fmaf(top, p.scale_log2e, shift));
-                    remainder = __any_sync(0xffffffffu, valid && most * 64.0f > l);
-                    if (lane == 0) remainder_flag[4 * tile + quad] = remainder ? 1u : 0u;
-                }
-                float sum0 = 0.0f, sum1 = 0.0f;
+                const float2 scale2 = make_float2(p.scale_log2e, p.scale_log2e), shift2 = make_float2(shift, shift);
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < G::kStep; c += 32) {
-                    uint32_t packed[16], rest[kRemainder ? 16 : 1];
+                    uint32_t packed[16];
 #pragma unroll
                     for (int i = 0; i < 16; ++i) {
-                        const float p0 = fast_exp2(fmaf(__uint_as_float(s[c + 2 * i]), p.scale_log2e, shift));
-                        const float p1 = fast_exp2(fmaf(__uint_as_float(s[c + 2 * i + 1]), p.scale_log2e, shift));
-                        sum0 += p0;
-                        sum1 += p1;
-                        packed[i] = pack2<T>(p0, p1);
-                        if constexpr (kRemainder) {
-                            rest[i] = 0u;
-                            if (remainder) {
-                                const float2 r = unpack2<T>(packed[i]);
-                                rest[i] = pack2<T>(p0 - r.x, p1 - r.y);
-                            }
-                        }
+                        float2 x = fma2(make_float2(__uint_as_float(s[c + 2 * i]), __uint_as_float(s[c + 2 * i + 1])), scale2, shift2);
+                        x.x = fast_exp2(x.x);
+                        x.y = fast_exp2(x.y);
+                        sum[i & 1] = add2(sum[i & 1], x);
+                        packed[i] = pack2<T>(x.x, x.y);
                     }
                     tmem_st16(s_at + c / 2, packed);
-                    // (zeros where another warp of the tile may ask for the second product)
-                    if constexpr (kRemainder) tmem_st16(s_at + 64 + c / 2, rest);
                 }
-                l += sum0 + sum1;
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                 tmem_st_wait();
                 tmem_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(p_full + 8 * tile);
+                if (lane == 0) mbar_arrive(p_full + 8 * (2 * tile + buffer));
             }
             if (!ok) break;
             // ---- epilogue
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN sum stays NaN)
             const uint64_t index = (uint64_t(tmpl) * p.num_q_heads + head) * p.max_q_tokens + row_tok;
             if (steps > 0) {
-                ok = mbar_wait_warp(o_full + 8 * tile, o_count & 1, abort_flag, p);
-                ++o_count;
+                ok = mbar_wait_warp(o_full + 8 * tile, done_tasks & 1, abort_flag, p);
+                ++done_tasks;
                 if (!ok) break;
                 tmem_fence_after();
             }

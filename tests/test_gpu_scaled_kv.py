@@ -280,7 +280,8 @@ def test_decode_matches_the_64_bit_restatement(device, code, io, hq, hkv, d, pag
 ])
 def test_several_tokens_match_the_64_bit_restatement(device, code, io, hq, hkv, d, page, histories, q_lens):
     case = make_scaled_case(hq * d, code, io, hq, hkv, d, histories, q_lens, page=page)
-    assert_close(ScaledRun(device, case, max_tokens=256).run(), *reference(case))
+    run = ScaledRun(device, case, max_tokens=256)
+    assert_close(run.run(), *reference(case, wide=run.wide()))
 
 
 def _wild(low, high):
@@ -536,7 +537,7 @@ def test_prefill_and_decode_in_one_call(device):
     tokens = len(case.q_bits)
     q = Buffer.from_slice(device, case.q_bits)
     mixed.record_sdpa(run.stream, q, run.pages, run.ids, Buffer.wrap(device, run.out.ref.ptr, tokens * run.row * 2))
-    assert_close(run.read(), *reference(case))
+    assert_close(run.read(), *reference(case, wide=True))
 
 
 # ---- wide Q tiles -----------------------------------------------------------------------------------------------------
@@ -553,9 +554,8 @@ def test_wide_tiles_match_the_64_bit_restatement(device, code, io, hq, hkv, page
     case = make_scaled_case(hq + page, code, io, hq, hkv, 128, histories, q_lens, page=page)
     run = ScaledRun(device, case, max_tokens=512)
     out = run.run()
-    execution = run.attention.metadata.variant().thread_block
-    assert execution.max_q_tokens * execution.max_q_heads > 32
-    assert_close(out, *reference(case))
+    assert run.wide()
+    assert_close(out, *reference(case, wide=True))
 
 
 @pytest.mark.parametrize("code", CODES)
@@ -565,7 +565,7 @@ def test_wide_tiles_over_rows_of_very_different_sizes(device, code, io, low, hig
     def some_zero(rng, tokens, heads):
         return _wild(low, high)(rng, tokens, heads) * (rng.random((tokens, heads)) > 0.2)
     case = make_scaled_case(80, code, io, 16, 2, 128, [200, 0], [64, 80], k_scale=_wild(-6, 1), v_scale=some_zero)
-    assert_close(ScaledRun(device, case, max_tokens=256).run(), *reference(case))
+    assert_close(ScaledRun(device, case, max_tokens=256).run(), *reference(case, wide=True))
 
 
 @pytest.mark.parametrize("code", CODES)
@@ -581,7 +581,7 @@ def test_wide_tiles_and_rows_that_are_not_finite(device, code, io):
     run.plan()
     run.record()
     out = run.read()
-    expected, bound = reference(case)
+    expected, bound = reference(case, wide=True)
     hidden = np.zeros(out.shape[:2], bool)
     hidden[30:64, 8:] = True
     assert np.isnan(out[hidden]).all()
@@ -608,6 +608,6 @@ def test_wide_tiles_with_windows(device, code, page):
         [case.slots[0]] * tokens, windows, [(0, 16), (16, 32)], [(0, 0, context), (1, 0, context)])]
     compute.invoke_direct(run.stream, sliced_q.DirectBuffers(run.q, run.pages, buffers[0], run.ids, *buffers[1:], run.out), 0, tokens, 2)
     out = run.read()
-    expected, bound = reference(case, [(0, b, e) for b, e in windows])
+    expected, bound = reference(case, [(0, b, e) for b, e in windows], wide=True)
     assert_close(out, expected, bound)
     assert not out[3].any()
