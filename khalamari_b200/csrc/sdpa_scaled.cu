@@ -22,9 +22,10 @@ static MapInstance make_chain_instance() {
     return MapInstance{sdpa_scaled_chain_kernel<T, CODE, D, NQ, W>, G::kThreads, G::kSmemBytes, G::kTileTokens, 16, G::kSlots, G::kRows};
 }
 
-template <typename T, int CODE>
+template <typename T, int CODE, int D>
 static MapInstance make_tc_instance() {
-    return MapInstance{sdpa_scaled_tc_kernel<T, CODE>, ScaledTc::kThreads, ScaledTc::kSmemBytes, ScaledTc::kStep, 16, ScaledTc::kRawSlots, 0};
+    using G = ScaledTc<D>;
+    return MapInstance{sdpa_scaled_tc_kernel<T, CODE, D>, G::kThreads, G::kSmemBytes, G::kStep, 16, G::kRawSlots, 0};
 }
 
 // Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM. Tasks wider than the widest
@@ -38,11 +39,12 @@ static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {
         if (rows <= 16) return make_stream_instance<T, CODE, 128, 2, 8, 1, 1>();
         if (rows <= 24) return make_chain_instance<T, CODE, 128, 3, 8>();
         if (rows <= 32) return make_chain_instance<T, CODE, 128, 4, 8>();
-        return make_tc_instance<T, CODE>();
+        return make_tc_instance<T, CODE, 128>();
     } else {
         if (rows <= 8) return make_stream_instance<T, CODE, 256, 1, 8, 1, 1>();
         if (rows <= 16) return make_chain_instance<T, CODE, 256, 2, 8>();
-        return make_chain_instance<T, CODE, 256, 3, 8>();
+        if (rows <= 24) return make_chain_instance<T, CODE, 256, 3, 8>();
+        return make_tc_instance<T, CODE, 256>();
     }
 }
 

@@ -1,13 +1,13 @@
-// Attention over scaled 8-bit pages (scaled_kv.cuh) for wide Q tiles (prefill, up to 128 rows a task) at head_dim 128, on
-// the 5th-generation tensor cores.
+// Attention over scaled 8-bit pages (scaled_kv.cuh) for wide Q tiles (prefill, up to 128 rows a task) on the
+// 5th-generation tensor cores.
 //
 //   S = Q K^T    tcgen05.mma kind::f16, M = 128 rows, N = 64 tokens; Q and K in shared memory, S in tensor memory.
 //   O += P V     P from tensor memory (over the columns of the S it came from), V in shared memory, O in tensor memory.
 //
 // Codes become 16-bit operands of the Q/output type once per step of 64 tokens, in shared memory, with their row's
 // power-of-two scale already applied: int8 and E4M3 codes times 2^e are exact in bf16, and in f16 as far as its range goes
-// (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). Two Q tiles of the same
-// sequence and KV head share every converted step. A probability is rounded to the Q/output type: in bf16 that is off by
+// (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). At head_dim 128 two Q tiles of
+// the same sequence and KV head share every converted step (at 256 tensor memory holds the output of one). A probability is rounded to the Q/output type: in bf16 that is off by
 // at most 2^-8, no more than what the cache rounds off a V element (2^-8 to 2^-7 of the row's largest).
 //
 // Each tile has two score buffers, so that the scores of step j + 1 are computed while the softmax of step j runs and the
@@ -17,8 +17,8 @@
 // two products of such a block take; and the issue slots, of which the conversion needs about as many as the softmax of
 // one tile - hence the two tiles per conversion.
 //
-// Warps: 0-3 softmax and epilogue of tile A (one thread a row), 4-7 of tile B, 8-12 conversion, 13 and 15 tensor-core
-// issue (one lane, a warp for each tile), 14 task decoding and copies. All waits are bounded (mbar_wait); no named
+// Warps: 0-3 softmax and epilogue of tile A (one thread a row), 4-7 of tile B (head_dim 256: conversion), 8-12
+// conversion, 13 and 15 tensor-core issue (one lane, a warp for each tile), 14 task decoding and copies. All waits are bounded (mbar_wait); no named
 // barriers between roles.
 #pragma once
 
@@ -29,20 +29,27 @@
 
 namespace kh {
 
+template <int D>
 struct ScaledTc {
-    static constexpr int kD = 128;
+    static_assert(D == 128 || D == 256, "head_dim 128 or 256");
+    static constexpr int kTiles = D == 128 ? 2 : 1;              // Q tiles at a time: O takes D columns of tensor memory
     static constexpr int kRows = 128;
     static constexpr int kStep = 64;                             // tokens of a step
-    static constexpr int kStages = 4;                            // steps of K and of V in shared memory
+    static constexpr int kStages = D == 128 ? 4 : 2;             // steps of K and of V in shared memory
     static constexpr int kChunks = kStep / 16;                   // raw slots (16 tokens) of a step
-    static constexpr int kRawSlots = 8;
-    static constexpr int kRawBytes = 2 * 16 * kD;
-    // a step's K or V, and a Q tile: two 64-element halves of [rows][128 bytes], 128-byte swizzle
-    static constexpr int kOperandBytes = kStep * kD * 2, kHalfBytes = kOperandBytes / 2;
-    static constexpr int kQBytes = kRows * kD * 2, kQHalfBytes = kQBytes / 2;
-    static constexpr int kConverters = 5;
+    static constexpr int kRawSlots = D == 128 ? 8 : 4;
+    static constexpr int kLines = D / 128;                       // 128-byte lines of a stored row
+    static constexpr int kRawBytes = 2 * 16 * D;
+    // a step's K or V, and a Q tile: groups of 64 elements, each [rows][128 bytes] with the 128-byte swizzle
+    static constexpr int kGroupBytes = kStep * 128, kOperandBytes = D / 64 * kGroupBytes;
+    static constexpr int kQGroupBytes = kRows * 128, kQBytes = D / 64 * kQGroupBytes;
+    static constexpr int kSoftmaxWarps = 4 * kTiles;
+    // Conversion warps take (chunk, K or V) units in turn. None is ever more than a ring of raw slots ahead of the others,
+    // so a wait on a slot cannot return on the phase before.
+    static constexpr int kConverters = D == 128 ? 5 : 8;
+    static_assert(kConverters <= 13 - kSoftmaxWarps && kConverters <= 2 * kRawSlots, "conversion warps");
     static constexpr int kThreads = 16 * 32;
-    static constexpr int kSmemBytes = 2 * kQBytes + 2 * kStages * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
+    static constexpr int kSmemBytes = kTiles * kQBytes + 2 * kStages * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
 
@@ -84,17 +91,16 @@ __device__ __forceinline__ bool elect_one() {
     return elected != 0;
 }
 
-template <typename T, int CODE>
-__global__ void __launch_bounds__(ScaledTc::kThreads, 1)
+template <typename T, int CODE, int D>
+__global__ void __launch_bounds__(ScaledTc<D>::kThreads, 1)
 sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap, const MapParams p) {
-    using G = ScaledTc;
-    constexpr int D = G::kD;
+    using G = ScaledTc<D>;
     constexpr float kRescaleLog2 = 8.0f;  // O is rescaled only when a row maximum grows by more than 2^8
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint8_t* const q_tile = smem;                                  // [2]
-    uint8_t* const k_ring = smem + 2 * G::kQBytes;                 // [kStages]
+    uint8_t* const q_tile = smem;                                  // [kTiles]
+    uint8_t* const k_ring = smem + G::kTiles * G::kQBytes;         // [kStages]
     uint8_t* const v_ring = k_ring + G::kStages * G::kOperandBytes;
     uint8_t* const raw_ring = v_ring + G::kStages * G::kOperandBytes;  // [kRawSlots]
     uint8_t* const raw_scales = raw_ring + G::kRawSlots * G::kRawBytes;
@@ -116,13 +122,13 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     if (tid == 0) {
         for (int i = 0; i < G::kRawSlots; ++i) {
             mbar_init(raw_full + 8 * i, 1);
-            mbar_init(raw_empty + 8 * i, 1);
+            mbar_init(raw_empty + 8 * i, 2);  // its K and its V have been converted
         }
         for (int i = 0; i < 4; ++i) {
             mbar_init(k_full + 8 * i, G::kChunks);
             mbar_init(v_full + 8 * i, G::kChunks);
-            mbar_init(k_empty + 8 * i, 2);
-            mbar_init(v_empty + 8 * i, 2);
+            mbar_init(k_empty + 8 * i, G::kTiles);
+            mbar_init(v_empty + 8 * i, G::kTiles);
             mbar_init(s_full + 8 * i, 1);
             mbar_init(p_full + 8 * i, 4);
         }
@@ -132,9 +138,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             mbar_init(o_free + 8 * i, 4);
             mbar_init(pv_done + 8 * i, 1);
             mbar_init(task_full + 8 * i, 1);
-            mbar_init(task_empty + 8 * i, 8 + G::kConverters + 2);
+            mbar_init(task_empty + 8 * i, G::kSoftmaxWarps + G::kConverters + G::kTiles);
         }
-        mbar_init(drain, 2);
+        mbar_init(drain, G::kTiles);
         *abort_flag = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -150,7 +156,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const ActiveCounts a = resolve_active(p);
 
-    if (warp >= 8) {
+    if (warp >= uint32_t(G::kSoftmaxWarps)) {
         if (warp == 14) {
             // ------------------------------ tasks and copies --------------------------------------------------------
             // Tasks are pairs of neighbouring templates, dealt round robin KV head by KV head, so that at any moment the
@@ -158,7 +164,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             // long rows of a causal batch do not come last.
             const uint32_t cells = p.num_kv_heads * p.head_ranges;
             // (few tasks: one tile each, on as many SMs)
-            const uint32_t stride = uint64_t(a.templates) * cells >= 2 * uint64_t(gridDim.x) ? 2 : 1;
+            const uint32_t stride = G::kTiles == 2 && uint64_t(a.templates) * cells >= 2 * uint64_t(gridDim.x) ? 2 : 1;
             const uint32_t pairs = (a.templates + stride - 1) / stride;
             const uint64_t total = uint64_t(pairs) * cells;
             const uint32_t page_shift = 31 - __clz(int(p.tokens_per_page));
@@ -311,14 +317,20 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         if (ok) {
                             const uint32_t bar = raw_full + 8 * slot, dst = smem_addr(raw_ring) + slot * G::kRawBytes;
                             const uint32_t sdst = smem_addr(raw_scales) + slot * 32;
+                            const uint32_t in_page = (first + x * 16) & (p.tokens_per_page - 1);  // (8-token pages: 0)
+                            const int32_t page_row = int32_t((kv_head << page_shift) + in_page);
+                            const uint8_t* const s0 = p.kv_pages + uint64_t(first_page) * p.page_bytes + scales + in_page;
                             mbar_arrive_expect_tx(bar, G::kRawBytes + 32);
-                            tma_load_5d(dst, &kv_map, int32_t(kv_head << page_shift), int32_t(first_page), bar, policy);
+                            tma_load_5d(dst, &kv_map, page_row, int32_t(first_page), bar, policy);
                             if (page_shift == 3) {
-                                tma_load_5d(dst + G::kRawBytes / 2, &kv_map, int32_t(kv_head << page_shift), int32_t(second_page), bar, policy);
-                                bulk_load(sdst, p.kv_pages + uint64_t(first_page) * p.page_bytes + scales, 16, bar);
+                                tma_load_5d(dst + G::kRawBytes / 2, &kv_map, page_row, int32_t(second_page), bar, policy);
+                                bulk_load(sdst, s0, 16, bar);
                                 bulk_load(sdst + 16, p.kv_pages + uint64_t(second_page) * p.page_bytes + scales, 16, bar);
-                            } else {
-                                bulk_load(sdst, p.kv_pages + uint64_t(first_page) * p.page_bytes + scales, 32, bar);
+                            } else if (page_shift == 4) {
+                                bulk_load(sdst, s0, 32, bar);
+                            } else {  // half of a 32-token page: its K and its V bytes
+                                bulk_load(sdst, s0, 16, bar);
+                                bulk_load(sdst + 16, s0 + p.tokens_per_page, 16, bar);
                             }
                         }
                     }
@@ -336,117 +348,120 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     }
                 }
             }
-        } else if (warp >= 8 + G::kConverters) {
+        } else if (warp >= 13) {
             // ------------------------------ tensor-core issue: a warp for each tile, one lane issues ------------------
             const uint32_t tile = warp == 15 ? 1 : 0;
-            constexpr uint32_t kFormat = umma_format<T>();
-            constexpr uint32_t idesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
-            constexpr uint32_t idesc_qk = idesc | ((uint32_t(G::kStep) >> 3) << 17);
-            constexpr uint32_t idesc_pv = idesc | ((uint32_t(D) >> 3) << 17) | (1u << 16);  // V: head dimension innermost
-            const uint64_t k_desc0 = umma_smem_desc(0, 16, 1024);
-            const uint64_t v_desc0 = umma_smem_desc(0, G::kHalfBytes, 1024);
-            const uint64_t q_desc = k_desc0 + uint64_t((smem_addr(q_tile) + tile * G::kQBytes) >> 4);
-            const uint32_t k_addr = smem_addr(k_ring), v_addr = smem_addr(v_ring);
-            const uint32_t scores = tmem_s + 128 * tile, out = tmem_o + 128 * tile;
-            uint32_t step = 0;                              // running step number of the K and V rings
-            uint32_t mine = 0;                              // running step number of this tile
-            uint32_t done_tasks = 0;                        // of this tile
-            bool ok = true;
-            auto stage_wait = [&](uint32_t bar, uint32_t number) {
-                return mbar_wait_warp(bar + 8 * (number % G::kStages), (number / G::kStages) & 1, abort_flag, p);
-            };
-            // scores of step `ahead` steps on, into their buffer
-            auto issue_scores = [&](uint32_t ahead) {
-                tmem_fence_after();
-                const uint32_t stage = (step + ahead) % G::kStages, buffer = (mine + ahead) & 1;
-                const uint64_t k = k_desc0 + uint64_t((k_addr + stage * G::kOperandBytes) >> 4);
-                if (elect_one()) {
-#pragma unroll
-                    for (int kk = 0; kk < D / 16; ++kk) {
-                        umma_ss(scores + 64 * buffer, q_desc + uint64_t(((kk / 4) * G::kQHalfBytes + (kk % 4) * 32) >> 4),
-                                k + uint64_t(((kk / 4) * G::kHalfBytes + (kk % 4) * 32) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
-                    }
-                    umma_commit(s_full + 8 * (2 * tile + buffer));
-                    umma_commit(k_empty + 8 * stage);
-                }
-                __syncwarp();
-            };
-            for (uint32_t taken = 0; ok; ++taken) {
-                const uint32_t ts = taken & 1;
-                if (!mbar_wait_warp(task_full + 8 * ts, (taken >> 1) & 1, abort_flag, p)) break;
-                if (tasks[ts].done) break;
-                const uint32_t steps = tasks[ts].steps;
-                const bool here = tile == 0 || tasks[ts].active_b != 0;
-                __syncwarp();
-                if (lane == 0) mbar_arrive(task_empty + 8 * ts);
-                if (!here) {
-                    // the steps pass by: this warp's arrivals on their slots
-                    for (uint32_t j = 0; j < steps && ok; ++j, ++step) {
-                        ok = stage_wait(k_full, step) && stage_wait(v_full, step);
-                        if (ok && lane == 0) {
-                            mbar_arrive(k_empty + 8 * (step % G::kStages));
-                            mbar_arrive(v_empty + 8 * (step % G::kStages));
-                        }
-                    }
-                    continue;
-                }
-                if (steps == 0) continue;
-                ok = mbar_wait_warp(q_full + 8 * tile, done_tasks & 1, abort_flag, p) && stage_wait(k_full, step);
-                if (!ok) break;
-                // (both buffers are free: every product of the task before has been waited for)
-                issue_scores(0);
-                if (steps > 1) {
-                    ok = stage_wait(k_full, step + 1);
-                    if (!ok) break;
-                    issue_scores(1);
-                }
-                for (uint32_t j = 0; j < steps && ok; ++j, ++step, ++mine) {
-                    // step j: the product with V, then the scores of step j + 2, which go where its probabilities lie
-                    const uint32_t buffer = mine & 1;
-                    ok = mbar_wait_warp(p_full + 8 * (2 * tile + buffer), (mine >> 1) & 1, abort_flag, p) && stage_wait(v_full, step);
-                    // the tile's first product overwrites O: its last epilogue must have read it
-                    if (ok && j == 0) ok = mbar_wait_warp(o_free + 8 * tile, (done_tasks & 1) ^ 1, abort_flag, p);
-                    if (!ok) break;
+            if (tile < uint32_t(G::kTiles)) {
+                constexpr uint32_t kFormat = umma_format<T>();
+                constexpr uint32_t idesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
+                constexpr uint32_t idesc_qk = idesc | ((uint32_t(G::kStep) >> 3) << 17);
+                constexpr uint32_t idesc_pv = idesc | ((uint32_t(D) >> 3) << 17) | (1u << 16);  // V: head dimension innermost
+                const uint64_t k_desc0 = umma_smem_desc(0, 16, 1024);
+                const uint64_t v_desc0 = umma_smem_desc(0, G::kGroupBytes, 1024);
+                const uint64_t q_desc = k_desc0 + uint64_t((smem_addr(q_tile) + tile * G::kQBytes) >> 4);
+                const uint32_t k_addr = smem_addr(k_ring), v_addr = smem_addr(v_ring);
+                const uint32_t scores = tmem_s + 128 * tile, out = tmem_o + 128 * tile;
+                uint32_t step = 0;                              // running step number of the K and V rings
+                uint32_t mine = 0;                              // running step number of this tile
+                uint32_t done_tasks = 0;                        // of this tile
+                bool ok = true;
+                auto stage_wait = [&](uint32_t bar, uint32_t number) {
+                    return mbar_wait_warp(bar + 8 * (number % G::kStages), (number / G::kStages) & 1, abort_flag, p);
+                };
+                // scores of step `ahead` steps on, into their buffer
+                auto issue_scores = [&](uint32_t ahead) {
                     tmem_fence_after();
-                    const uint32_t stage = step % G::kStages;
-                    const uint64_t v = v_desc0 + uint64_t((v_addr + stage * G::kOperandBytes) >> 4);
+                    const uint32_t stage = (step + ahead) % G::kStages, buffer = (mine + ahead) & 1;
+                    const uint64_t k = k_desc0 + uint64_t((k_addr + stage * G::kOperandBytes) >> 4);
                     if (elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < G::kStep / 16; ++i) {
-                            umma_ts(out, scores + 64 * buffer + 8 * i, v + uint64_t((i * 2048) >> 4), idesc_pv, j > 0 || i > 0 ? 1u : 0u);
+                        for (int kk = 0; kk < D / 16; ++kk) {
+                            umma_ss(scores + 64 * buffer, q_desc + uint64_t(((kk / 4) * G::kQGroupBytes + (kk % 4) * 32) >> 4),
+                                    k + uint64_t(((kk / 4) * G::kGroupBytes + (kk % 4) * 32) >> 4), idesc_qk, kk > 0 ? 1u : 0u);
                         }
-                        umma_commit(pv_done + 8 * tile);
-                        umma_commit(v_empty + 8 * stage);
-                        if (j + 1 == steps) umma_commit(o_full + 8 * tile);
+                        umma_commit(s_full + 8 * (2 * tile + buffer));
+                        umma_commit(k_empty + 8 * stage);
                     }
                     __syncwarp();
-                    if (j + 2 < steps) ok = stage_wait(k_full, step + 2);
-                    ok = ok && mbar_wait_warp(pv_done + 8 * tile, mine & 1, abort_flag, p);
+                };
+                for (uint32_t taken = 0; ok; ++taken) {
+                    const uint32_t ts = taken & 1;
+                    if (!mbar_wait_warp(task_full + 8 * ts, (taken >> 1) & 1, abort_flag, p)) break;
+                    if (tasks[ts].done) break;
+                    const uint32_t steps = tasks[ts].steps;
+                    const bool here = tile == 0 || tasks[ts].active_b != 0;
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(task_empty + 8 * ts);
+                    if (!here) {
+                        // the steps pass by: this warp's arrivals on their slots
+                        for (uint32_t j = 0; j < steps && ok; ++j, ++step) {
+                            ok = stage_wait(k_full, step) && stage_wait(v_full, step);
+                            if (ok && lane == 0) {
+                                mbar_arrive(k_empty + 8 * (step % G::kStages));
+                                mbar_arrive(v_empty + 8 * (step % G::kStages));
+                            }
+                        }
+                        continue;
+                    }
+                    if (steps == 0) continue;
+                    ok = mbar_wait_warp(q_full + 8 * tile, done_tasks & 1, abort_flag, p) && stage_wait(k_full, step);
                     if (!ok) break;
-                    if (j + 2 < steps) issue_scores(2);
+                    // (both buffers are free: every product of the task before has been waited for)
+                    issue_scores(0);
+                    if (steps > 1) {
+                        ok = stage_wait(k_full, step + 1);
+                        if (!ok) break;
+                        issue_scores(1);
+                    }
+                    for (uint32_t j = 0; j < steps && ok; ++j, ++step, ++mine) {
+                        // step j: the product with V, then the scores of step j + 2, which go where its probabilities lie
+                        const uint32_t buffer = mine & 1;
+                        ok = mbar_wait_warp(p_full + 8 * (2 * tile + buffer), (mine >> 1) & 1, abort_flag, p) && stage_wait(v_full, step);
+                        // the tile's first product overwrites O: its last epilogue must have read it
+                        if (ok && j == 0) ok = mbar_wait_warp(o_free + 8 * tile, (done_tasks & 1) ^ 1, abort_flag, p);
+                        if (!ok) break;
+                        tmem_fence_after();
+                        const uint32_t stage = step % G::kStages;
+                        const uint64_t v = v_desc0 + uint64_t((v_addr + stage * G::kOperandBytes) >> 4);
+                        if (elect_one()) {
+#pragma unroll
+                            for (int i = 0; i < G::kStep / 16; ++i) {
+                                umma_ts(out, scores + 64 * buffer + 8 * i, v + uint64_t((i * 2048) >> 4), idesc_pv, j > 0 || i > 0 ? 1u : 0u);
+                            }
+                            umma_commit(pv_done + 8 * tile);
+                            umma_commit(v_empty + 8 * stage);
+                            if (j + 1 == steps) umma_commit(o_full + 8 * tile);
+                        }
+                        __syncwarp();
+                        if (j + 2 < steps) ok = stage_wait(k_full, step + 2);
+                        ok = ok && mbar_wait_warp(pv_done + 8 * tile, mine & 1, abort_flag, p);
+                        if (!ok) break;
+                        if (j + 2 < steps) issue_scores(2);
+                    }
+                    ++done_tasks;
                 }
-                ++done_tasks;
+                // nothing issued here may still be running when tensor memory is freed (bounded, also on the abort path)
+                if (elect_one()) umma_commit(drain);
+                __syncwarp();
+                for (uint32_t i = 0; i < p.wait_limit; ++i) {
+                    if (mbar_try_wait(drain, 0)) break;
+                }
             }
-            // nothing issued here may still be running when tensor memory is freed (bounded, also on the abort path)
-            if (elect_one()) umma_commit(drain);
-            __syncwarp();
-            for (uint32_t i = 0; i < p.wait_limit; ++i) {
-                if (mbar_try_wait(drain, 0)) break;
-            }
-        } else {
+        } else if (warp < uint32_t(G::kSoftmaxWarps + G::kConverters)) {
             // ------------------------------ conversion ---------------------------------------------------------------
-            // A warp takes every kConverters-th 16-token chunk. Eight consecutive lanes take the lower four 16-byte pieces
-            // of one row and the upper four of its neighbour: that makes their loads, and both rounds of their 16-byte
-            // stores, touch every bank once (128-byte swizzle on both sides).
+            // A warp takes every kConverters-th unit: the K or the V rows of a 16-token chunk. Eight consecutive lanes take the
+            // lower four 16-byte pieces of one row and the upper four of its neighbour: that makes their loads, and both
+            // rounds of their 16-byte stores, touch every bank once (128-byte swizzle on both sides).
             const uint32_t sub = (lane >> 2) & 1, cc = lane & 3, row_pair = lane >> 4, flip = (lane >> 3) & 1;
             const uint32_t row4 = 2 * row_pair + (sub ^ flip), piece = 4 * sub + cc;
-            // Rows 4 i + row4, i < 4. A copy holds [K/V][16 rows], or two of [K/V][8 rows] (8-token pages); scale bytes alike.
+            // Rows 4 i + row4, i < 4. A copy holds [K/V][line][16 rows], or two of [K/V][line][8 rows] (8-token pages); scale
+            // bytes alike, without lines.
             const bool short_pages = p.tokens_per_page == 8;
             const uint32_t in_lane = row4 * 128 + ((piece ^ row4) << 4);
-            const uint32_t out_lane = sub * G::kHalfBytes + row4 * 128 + (((2 * cc) ^ row4) << 4);
-            const uint32_t plane_stride = short_pages ? 1024 : 2048, half_stride = short_pages ? 2048 : 1024;
+            const uint32_t out_lane = sub * G::kGroupBytes + row4 * 128 + (((2 * cc) ^ row4) << 4);
+            const uint32_t line_stride = short_pages ? 1024 : 2048, half_stride = short_pages ? G::kRawBytes / 2 : 1024;
             const uint32_t scale_plane = short_pages ? 8 : 16, scale_half = short_pages ? 16 : 8;
-            uint32_t step = 0, raw = 0, chunk_number = 0;  // running numbers
+            uint32_t step = 0, raw = 0, unit = 0;  // running numbers
             bool ok = true;
             for (uint32_t taken = 0; ok; ++taken) {
                 const uint32_t ts = taken & 1;
@@ -456,8 +471,11 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 __syncwarp();
                 if (lane == 0) mbar_arrive(task_empty + 8 * ts);
                 const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
-                for (uint32_t x = 0; x < steps * G::kChunks && ok; ++x, ++chunk_number) {
-                    if (chunk_number % G::kConverters != warp - 8) continue;
+                const uint32_t units = steps * G::kChunks * 2;
+                // this warp's first unit of the task
+                for (uint32_t u = (warp - G::kSoftmaxWarps + G::kConverters - unit % G::kConverters) % G::kConverters; u < units && ok;
+                     u += G::kConverters) {
+                    const uint32_t x = u >> 1, plane = u & 1;
                     const uint32_t number = step + x / G::kChunks, stage = number % G::kStages, phase = (number / G::kStages) & 1;
                     const uint32_t raw_number = raw + x, slot = raw_number % G::kRawSlots;
                     const bool there = x < slots;
@@ -466,16 +484,16 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     const uint8_t* const scales = raw_scales + slot * 32 + row4;
                     const uint32_t token = first + x * 16;
                     const bool whole = there && token >= begin && token + 16 <= end;
+                    ok = ok && mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
+                    if (!ok) break;
+                    uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
 #pragma unroll
-                    for (int plane = 0; plane < 2; ++plane) {
-                        ok = ok && mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
-                        if (!ok) break;
-                        uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
+                    for (int line = 0; line < G::kLines; ++line) {
                         uint4 words[4];
                         uint32_t b[4];
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t at = plane * plane_stride + (i >> 1) * half_stride + (i & 1) * 512;
+                            const uint32_t at = (plane * G::kLines + line) * line_stride + (i >> 1) * half_stride + (i & 1) * 512;
                             words[i] = *reinterpret_cast<const uint4*>(source + at + (in_lane ^ ((i & 1) * 64)));
                             b[i] = scales[plane * scale_plane + (i >> 1) * scale_half + (i & 1) * 4];
                         }
@@ -510,16 +528,19 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                                 for (int w = 0; w < 8; ++w) r[w] = saturate2<T>(r[w]);
                             }
                             // rows 4-7 of an eight-row swizzle period: position bit 2 flips
-                            uint8_t* const row = out + i * 512;
+                            uint8_t* const row = out + line * 2 * G::kGroupBytes + i * 512;
                             *reinterpret_cast<uint4*>(row + (out_lane ^ ((i & 1) * 64))) = make_uint4(r[0], r[1], r[2], r[3]);
                             *reinterpret_cast<uint4*>(row + (out_lane ^ ((i & 1) * 64) ^ 16)) = make_uint4(r[4], r[5], r[6], r[7]);
                         }
-                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
                     }
-                    if (ok && there && lane == 0) mbar_arrive(raw_empty + 8 * slot);
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
+                        if (there) mbar_arrive(raw_empty + 8 * slot);
+                    }
                 }
+                unit += units;
                 step += steps;
                 raw += slots;
             }
@@ -556,9 +577,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 uint8_t* const dst = q_tile + tile * G::kQBytes + row * 128;
                 const uint4* const src = reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + q_row * D);
 #pragma unroll
-                for (int c = 0; c < 16; ++c) {
+                for (int c = 0; c < D / 8; ++c) {
                     const uint4 v = valid ? src[c] : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4*>(dst + (c / 8) * G::kQHalfBytes + (((c % 8) ^ (row & 7)) << 4)) = v;
+                    *reinterpret_cast<uint4*>(dst + (c / 8) * G::kQGroupBytes + (((c % 8) ^ (row & 7)) << 4)) = v;
                 }
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();

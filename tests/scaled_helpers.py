@@ -136,8 +136,8 @@ def reference(case: ScaledCase, visible=None, wide: bool = False) -> tuple[np.nd
     """(attention output, per-element error bound) in 64 bits.
 
     The bound counts what the kernels round: the output, half a step of its type; the value weights, to f16 (half a
-    step: 2^-11 of each term; 2^-8 where a ``wide`` Q tile, of more than 32 rows at head_dim 128, has bf16
-    probabilities), plus 2^-25 of the largest weight where a weight is subnormal there - references lie at
+    step: 2^-11 of each term; 2^-8 where a ``wide`` Q tile, of more than 32 rows (24 at head_dim 256), has
+    bf16 probabilities), plus 2^-25 of the largest weight where a weight is subnormal there - references lie at
     most 2^8 below the largest weight, and a code is at most twice the row's largest code, so 2^-25 * 2 * largest
     |p v| per token); and f32 arithmetic on the scores: a dot product of D terms is off by at most D * 2^-23 of the
     sum of magnitudes (additions that may truncate), a handful of roundings of the score and of exp2 add 2^-20 of
@@ -212,7 +212,7 @@ class ScaledRun:
 
     def wide(self) -> bool:
         block = self.attention.metadata.variant().thread_block
-        return self.case.d == 128 and block.max_q_tokens * block.max_q_heads > 32
+        return block.max_q_tokens * block.max_q_heads > (32 if self.case.d == 128 else 24)
 
     def read(self):
         self.stream.synchronize()

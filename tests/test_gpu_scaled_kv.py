@@ -543,15 +543,19 @@ def test_prefill_and_decode_in_one_call(device):
 # ---- wide Q tiles -----------------------------------------------------------------------------------------------------
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("io", ["bf16", "f16"])
-@pytest.mark.parametrize("hq,hkv,page,histories,q_lens", [
-    (16, 2, 16, [700, 0, 133], [200, 129, 49]),   # odd numbers of tiles: pairs that straddle two requests
-    (32, 8, 8, [300], [333]),                     # a group of four heads, 32-token tiles
-    (12, 2, 16, [61, 5], [97, 64]),               # a group of six: 96 of 128 rows
-    (8, 1, 16, [2000], [40]),                     # few tiles: the KV range is cut
-    (5, 1, 8, [0], [300]),
+@pytest.mark.parametrize("d,hq,hkv,page,histories,q_lens", [
+    (128, 16, 2, 16, [700, 0, 133], [200, 129, 49]),   # odd numbers of tiles: pairs that straddle two requests
+    (128, 32, 8, 8, [300], [333]),                     # a group of four heads, 32-token tiles
+    (128, 12, 2, 16, [61, 5], [97, 64]),               # a group of six: 96 of 128 rows
+    (128, 8, 1, 16, [2000], [40]),                     # few tiles: the KV range is cut
+    (128, 5, 1, 8, [0], [300]),
+    (256, 16, 2, 16, [300, 0], [100, 33]),
+    (256, 12, 2, 8, [61, 5], [97, 64]),
+    (256, 4, 4, 32, [200], [170]),
+    (256, 8, 1, 32, [1500], [24]),
 ])
-def test_wide_tiles_match_the_64_bit_restatement(device, code, io, hq, hkv, page, histories, q_lens):
-    case = make_scaled_case(hq + page, code, io, hq, hkv, 128, histories, q_lens, page=page)
+def test_wide_tiles_match_the_64_bit_restatement(device, code, io, d, hq, hkv, page, histories, q_lens):
+    case = make_scaled_case(hq + page, code, io, hq, hkv, d, histories, q_lens, page=page)
     run = ScaledRun(device, case, max_tokens=512)
     out = run.run()
     assert run.wide()
@@ -559,20 +563,22 @@ def test_wide_tiles_match_the_64_bit_restatement(device, code, io, hq, hkv, page
 
 
 @pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("d", [128, 256])
 @pytest.mark.parametrize("io,low,high", [("bf16", -40, 40), ("f16", -14, 11)])
-def test_wide_tiles_over_rows_of_very_different_sizes(device, code, io, low, high):
+def test_wide_tiles_over_rows_of_very_different_sizes(device, code, d, io, low, high):
     """V rows whose scales differ by up to 2^80 (f16: up to its whole range), some of them zero."""
     def some_zero(rng, tokens, heads):
         return _wild(low, high)(rng, tokens, heads) * (rng.random((tokens, heads)) > 0.2)
-    case = make_scaled_case(80, code, io, 16, 2, 128, [200, 0], [64, 80], k_scale=_wild(-6, 1), v_scale=some_zero)
+    case = make_scaled_case(80, code, io, 16, 2, d, [200, 0], [64, 80], k_scale=_wild(-6, 1), v_scale=some_zero)
     assert_close(ScaledRun(device, case, max_tokens=256).run(), *reference(case, wide=True))
 
 
 @pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("io", ["bf16", "f16"])
-def test_wide_tiles_and_rows_that_are_not_finite(device, code, io):
-    case = make_scaled_case(81, code, io, 16, 2, 128, [300, 150], [64, 40])
-    codes, scales = planes(case.pool, 2, 16, 128)
+@pytest.mark.parametrize("d", [128, 256])
+def test_wide_tiles_and_rows_that_are_not_finite(device, code, io, d):
+    case = make_scaled_case(81, code, io, 16, 2, d, [300, 150], [64, 40])
+    codes, scales = planes(case.pool, 2, 16, d)
     at = 330  # a token of request 0's own chunk, KV head 1: seen by its queries from number 30 on
     page = case.table[case.slots[0], 0, at // 16]
     scales[page, 1, :, at % 16] = 255
@@ -589,13 +595,13 @@ def test_wide_tiles_and_rows_that_are_not_finite(device, code, io):
 
 
 @pytest.mark.parametrize("code", CODES)
-@pytest.mark.parametrize("page", [8, 16])
-def test_wide_tiles_with_windows(device, code, page):
+@pytest.mark.parametrize("d,page", [(128, 8), (128, 16), (256, 8), (256, 32)])
+def test_wide_tiles_with_windows(device, code, d, page):
     """Direct output with per-token visible ranges: windows of different lengths, empty ones, unallocated pages below."""
     from khalamari_b200 import sliced_q
     from khalamari_b200.device import Buffer
     from khalamari_b200.sdpa import ExecutionVariant
-    hq, hkv, d, tokens, context = 16, 2, 128, 32, 500
+    hq, hkv, tokens, context = 16, 2, 32, 500
     case = make_scaled_case(82, code, "bf16", hq, hkv, d, [context - tokens], [tokens], page=page)
     case.table[case.slots[0], 0, :200 // page] = 0xFFFFFF00
     run = ScaledRun(device, case)
