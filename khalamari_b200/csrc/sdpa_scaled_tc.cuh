@@ -44,9 +44,14 @@ struct ScaledTc {
     static constexpr int kGroupBytes = kStep * 128, kOperandBytes = D / 64 * kGroupBytes;
     static constexpr int kQGroupBytes = kRows * 128, kQBytes = D / 64 * kQGroupBytes;
     static constexpr int kSoftmaxWarps = 4 * kTiles;
-    // Conversion warps take (chunk, K or V) units in turn. None is ever more than a ring of raw slots ahead of the others,
-    // so a wait on a slot cannot return on the phase before.
+    // Conversion warps take (chunk, K or V) units in turn. A wait tells a barrier's phases apart by their parity only, and a
+    // warp does not wait for every copy, nor do copies land in order; so every slot has two barriers used in turn. Then
+    // the phase before the one that a warp waits for belongs to copy r - 2 kRawSlots, which is known to have landed: the
+    // warp's last unit was of copy r - kRawSlots or a later one, that copy landed, hence r - kRawSlots had been issued (in
+    // order), hence r - 2 kRawSlots had left the slot. (Chunks past the end of a task count as copies: the distance between
+    // a warp's units is fixed.)
     static constexpr int kConverters = D == 128 ? 5 : 8;
+    static constexpr int kRawBars = 2 * kRawSlots;
     static_assert(kConverters <= 13 - kSoftmaxWarps && kConverters <= 2 * kRawSlots, "conversion warps");
     static constexpr int kThreads = 16 * 32;
     static constexpr int kSmemBytes = kTiles * kQBytes + 2 * kStages * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
@@ -107,13 +112,13 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     ScaledTcTask* const tasks = reinterpret_cast<ScaledTcTask*>(raw_scales + G::kRawSlots * 32);  // [2]
     uint64_t* const bars = reinterpret_cast<uint64_t*>(tasks + 2);
     const uint32_t bar0 = smem_addr(bars);
-    const uint32_t raw_full = bar0, raw_empty = bar0 + 64;         // [8] each
-    const uint32_t k_full = bar0 + 128, k_empty = bar0 + 160, v_full = bar0 + 192, v_empty = bar0 + 224;  // [4] each
-    const uint32_t s_full = bar0 + 256, p_full = bar0 + 288;       // [tile][buffer]
-    const uint32_t q_full = bar0 + 320, o_full = bar0 + 336, o_free = bar0 + 352, pv_done = bar0 + 368;  // [tile]
-    const uint32_t task_full = bar0 + 384, task_empty = bar0 + 400;  // [2]
-    const uint32_t drain = bar0 + 416;
-    constexpr int kBars = 53;
+    const uint32_t raw_empty = bar0;                               // [8]
+    const uint32_t k_full = bar0 + 64, k_empty = bar0 + 96, v_full = bar0 + 128, v_empty = bar0 + 160;  // [4] each
+    const uint32_t s_full = bar0 + 192, p_full = bar0 + 224;       // [tile][buffer]
+    const uint32_t q_full = bar0 + 256, o_full = bar0 + 272, o_free = bar0 + 288, pv_done = bar0 + 304;  // [tile]
+    const uint32_t task_full = bar0 + 320, task_empty = bar0 + 336;  // [2]
+    const uint32_t drain = bar0 + 352, raw_full = bar0 + 360;      // [1], [16]
+    constexpr int kBars = 61;
     volatile uint32_t* const abort_flag = reinterpret_cast<volatile uint32_t*>(bars + kBars);
     uint32_t* const tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
     static_assert(sizeof(ScaledTcTask) * 2 + kBars * 8 + 16 <= 1024, "small shared memory");
@@ -121,9 +126,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < G::kRawSlots; ++i) {
-            mbar_init(raw_full + 8 * i, 1);
             mbar_init(raw_empty + 8 * i, 2);  // its K and its V have been converted
         }
+        for (int i = 0; i < G::kRawBars; ++i) mbar_init(raw_full + 8 * i, 1);
         for (int i = 0; i < 4; ++i) {
             mbar_init(k_full + 8 * i, G::kChunks);
             mbar_init(v_full + 8 * i, G::kChunks);
@@ -294,10 +299,10 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 const uint32_t begin = task.begin, end = task.end, first = task.first, kv_head = task.kv_head;
                 const uint64_t table = (uint64_t(task.req_slot) * p.num_gqa_layers + p.layer_index) * p.pages_per_request_layer;
                 const uint64_t scales = uint64_t((p.num_kv_heads * 2) << page_shift) * D + ((kv_head * 2) << page_shift);
-                const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
+                const uint32_t slots = end > first ? (end - first + 15) / 16 : 0, chunks = task.steps * G::kChunks;
                 uint32_t page0 = 0, page1 = 0;
                 if (slots == 0) next_task();
-                for (uint32_t x = 0; x < slots && ok; ++x) {
+                for (uint32_t x = 0; x < chunks && ok; ++x) {
                     if ((x & 31) == 0 && x + lane < slots) {
                         const uint32_t token = first + (x + lane) * 16;
                         // (the first half may lie before everything that is visible, the second behind it)
@@ -314,8 +319,10 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     const uint32_t slot = issued % G::kRawSlots, phase = (issued / G::kRawSlots) & 1;
                     if (lane == 0) {
                         ok = mbar_wait(raw_empty + 8 * slot, phase ^ 1, abort_flag, p);
-                        if (ok) {
-                            const uint32_t bar = raw_full + 8 * slot, dst = smem_addr(raw_ring) + slot * G::kRawBytes;
+                        const uint32_t bar = raw_full + 8 * (issued % G::kRawBars);
+                        if (ok && x >= slots) mbar_arrive(bar);  // the last step's chunks past the end: nothing to copy
+                        if (ok && x < slots) {
+                            const uint32_t dst = smem_addr(raw_ring) + slot * G::kRawBytes;
                             const uint32_t sdst = smem_addr(raw_scales) + slot * 32;
                             const uint32_t in_page = (first + x * 16) & (p.tokens_per_page - 1);  // (8-token pages: 0)
                             const int32_t page_row = int32_t((kv_head << page_shift) + in_page);
@@ -344,7 +351,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 for (uint32_t back = 0; back < uint32_t(G::kRawSlots) && back < issued; ++back) {
                     const uint32_t c = issued - 1 - back;
                     for (uint32_t i = 0; i < p.wait_limit; ++i) {
-                        if (mbar_try_wait(raw_full + 8 * (c % G::kRawSlots), (c / G::kRawSlots) & 1)) break;
+                        if (mbar_try_wait(raw_full + 8 * (c % G::kRawBars), (c / G::kRawBars) & 1)) break;
                     }
                 }
             }
@@ -461,7 +468,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             const uint32_t out_lane = sub * G::kGroupBytes + row4 * 128 + (((2 * cc) ^ row4) << 4);
             const uint32_t line_stride = short_pages ? 1024 : 2048, half_stride = short_pages ? G::kRawBytes / 2 : 1024;
             const uint32_t scale_plane = short_pages ? 8 : 16, scale_half = short_pages ? 16 : 8;
-            uint32_t step = 0, raw = 0, unit = 0;  // running numbers
+            uint32_t step = 0, unit = 0;  // running numbers
             bool ok = true;
             for (uint32_t taken = 0; ok; ++taken) {
                 const uint32_t ts = taken & 1;
@@ -477,9 +484,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                      u += G::kConverters) {
                     const uint32_t x = u >> 1, plane = u & 1;
                     const uint32_t number = step + x / G::kChunks, stage = number % G::kStages, phase = (number / G::kStages) & 1;
-                    const uint32_t raw_number = raw + x, slot = raw_number % G::kRawSlots;
+                    const uint32_t raw_number = step * G::kChunks + x, slot = raw_number % G::kRawSlots;
                     const bool there = x < slots;
-                    if (there) ok = mbar_wait_warp(raw_full + 8 * slot, (raw_number / G::kRawSlots) & 1, abort_flag, p);
+                    ok = mbar_wait_warp(raw_full + 8 * (raw_number % G::kRawBars), (raw_number / G::kRawBars) & 1, abort_flag, p);
                     const uint8_t* const source = raw_ring + slot * G::kRawBytes;
                     const uint8_t* const scales = raw_scales + slot * 32 + row4;
                     const uint32_t token = first + x * 16;
@@ -537,12 +544,11 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     __syncwarp();
                     if (lane == 0) {
                         mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
-                        if (there) mbar_arrive(raw_empty + 8 * slot);
+                        mbar_arrive(raw_empty + 8 * slot);
                     }
                 }
                 unit += units;
                 step += steps;
-                raw += slots;
             }
         }
     } else {

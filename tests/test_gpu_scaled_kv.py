@@ -563,6 +563,23 @@ def test_wide_tiles_match_the_64_bit_restatement(device, code, io, d, hq, hkv, p
 
 
 @pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("d,hq,hkv,page", [(128, 32, 8, 16), (128, 32, 8, 8), (256, 16, 4, 16), (256, 16, 4, 32)])
+def test_many_ragged_wide_tiles_follow_one_another(device, code, d, hq, hkv, page):
+    """Several tasks a CTA, most of them ending inside a step, some within its first 16 tokens: rings run on from task to task."""
+    rng = np.random.default_rng(84)
+    q_lens = rng.integers(9, 48, 120).tolist()
+    histories = [0 if i % 4 == 0 else int(rng.integers(1, 200)) for i in range(120)]
+    case = make_scaled_case(85, code, "bf16", hq, hkv, d, histories, q_lens, page=page)
+    run = ScaledRun(device, case)
+    out = run.run()
+    assert run.wide()
+    assert_close(out, *reference(case, wide=True))
+    for _ in range(4):
+        run.record()
+        assert np.array_equal(out, run.read())
+
+
+@pytest.mark.parametrize("code", CODES)
 @pytest.mark.parametrize("d", [128, 256])
 @pytest.mark.parametrize("io,low,high", [("bf16", -40, 40), ("f16", -14, 11)])
 def test_wide_tiles_over_rows_of_very_different_sizes(device, code, d, io, low, high):
