@@ -540,9 +540,10 @@ static void launch_reduce(kh_dtype dtype, const ReduceParams& p, uint32_t num_ra
 
 // The map kernels of scaled pages leave one full partial per chain of slices among empty ones, so their lists are long
 // and mostly statistics. From 32 partials per range on, a row's list is shared by the thread groups of a wide block (one
-// sequence of 524,288 tokens in 1,024 slices: the reduce takes 150 us in one list, and a sixteenth of the steps here).
-static uint32_t wide_reduce(kh_dtype kv_dtype, uint32_t templates, uint32_t ranges) {
-    return is_scaled(kv_dtype) && templates / ranges >= 32 ? 1u : 0u;
+// sequence of 524,288 tokens in 1,024 slices: the reduce takes 150 us in one list, and a sixteenth of the steps here). A
+// wide block also takes the rows of a Q tile side by side where 128 threads would take them in turn.
+static uint32_t wide_reduce(kh_dtype kv_dtype, uint32_t templates, uint32_t ranges, uint32_t columns) {
+    return is_scaled(kv_dtype) && (templates / 32 >= ranges || columns > 4 * 128) ? 1u : 0u;
 }
 
 static void validate_layout(const kh_page_table_layout& l) {
@@ -1168,7 +1169,7 @@ kh_status kh_sliced_kv_reduce(kh_sliced_kv* compute, kh_stream* stream, const kh
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 0;
-        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens);
+        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens, p.head_dim);
         launch_reduce(compute->config.dtype, p, num_active_tokens, stream->stream);
         return KH_OK;
     });
@@ -1379,7 +1380,8 @@ kh_status kh_sliced_q_reduce(kh_sliced_q* compute, kh_stream* stream, const kh_s
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 1;
-        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_q_token_tiles);
+        p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_q_token_tiles,
+                             p.max_q_tokens * p.head_dim);
         launch_reduce(compute->config.dtype, p, num_active_q_token_tiles, stream->stream);
         return KH_OK;
     });

@@ -113,6 +113,19 @@ struct ScaledRows {
     }
 };
 
+// A wait of a whole warp: the same answer in every lane.
+__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, const MapParams& p) {
+    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p));
+}
+
+// One lane of a converged warp, the same one every time. Tensor-core instructions and bulk copies issued under it need no
+// handling of operands that differ between lanes, which under `lane == 0` costs each of them about a hundred cycles.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t elected;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(elected));
+    return elected != 0;
+}
+
 __device__ __forceinline__ void tma_load_5d(uint32_t dst, const CUtensorMap* map, int32_t row, int32_t page, uint32_t bar,
                                             uint64_t policy) {
     asm volatile(
@@ -403,36 +416,34 @@ struct ScaledFetch {
         }
         const uint32_t first_page = __shfl_sync(0xffffffffu, page0, int(i)), row = __shfl_sync(0xffffffffu, row0, int(i));
         const uint32_t second_page = __shfl_sync(0xffffffffu, page1, int(i));
-        bool ok = true;
-        if (lane == 0) {
-            ok = mbar_wait(empty_bar + 8 * slot, phase ^ 1, abort_flag, p);
-            if (ok) {
-                const uint32_t bar = full_bar + 8 * slot, dst = ring + slot * G::kSlotBytes, sdst = scales + slot * G::kScaleBytes;
-                const uint32_t P = p.tokens_per_page;
-                mbar_arrive_expect_tx(bar, G::kSlotBytes + G::kScaleBytes);
-                // scale bytes of the first head's K rows
-                const uint8_t* s0 = p.kv_pages + uint64_t(first_page) * p.page_bytes + uint64_t((p.num_kv_heads * 2) << page_shift) * D +
-                                    ((row >> page_shift << page_shift) * 2) + (row & (P - 1));
-                tma_load_5d(dst, map, int32_t(row), int32_t(first_page), bar, policy);
-                if (page_shift == 3) {  // two 8-token pages
-                    const uint8_t* s1 = s0 + (int64_t(second_page) - int64_t(first_page)) * p.page_bytes;
-                    tma_load_5d(dst + G::kSlotBytes / 2, map, int32_t(row), int32_t(second_page), bar, policy);
-                    bulk_load(sdst, s0, G::kScaleBytes / 2, bar);
-                    bulk_load(sdst + G::kScaleBytes / 2, s1, G::kScaleBytes / 2, bar);
-                } else if (page_shift == 4) {
-                    bulk_load(sdst, s0, G::kScaleBytes, bar);
-                } else {  // half of a 32-token page: its K and its V bytes
-                    bulk_load(sdst, s0, 16, bar);
-                    bulk_load(sdst + 16, s0 + P, 16, bar);
-                }
+        if (!mbar_wait_warp(empty_bar + 8 * slot, phase ^ 1, abort_flag, p)) return false;
+        if (elect_one()) {
+            const uint32_t bar = full_bar + 8 * slot, dst = ring + slot * G::kSlotBytes, sdst = scales + slot * G::kScaleBytes;
+            const uint32_t P = p.tokens_per_page;
+            mbar_arrive_expect_tx(bar, G::kSlotBytes + G::kScaleBytes);
+            // scale bytes of the first head's K rows
+            const uint8_t* s0 = p.kv_pages + uint64_t(first_page) * p.page_bytes + uint64_t((p.num_kv_heads * 2) << page_shift) * D +
+                                ((row >> page_shift << page_shift) * 2) + (row & (P - 1));
+            tma_load_5d(dst, map, int32_t(row), int32_t(first_page), bar, policy);
+            if (page_shift == 3) {  // two 8-token pages
+                const uint8_t* s1 = s0 + (int64_t(second_page) - int64_t(first_page)) * p.page_bytes;
+                tma_load_5d(dst + G::kSlotBytes / 2, map, int32_t(row), int32_t(second_page), bar, policy);
+                bulk_load(sdst, s0, G::kScaleBytes / 2, bar);
+                bulk_load(sdst + G::kScaleBytes / 2, s1, G::kScaleBytes / 2, bar);
+            } else if (page_shift == 4) {
+                bulk_load(sdst, s0, G::kScaleBytes, bar);
+            } else {  // half of a 32-token page: its K and its V bytes
+                bulk_load(sdst, s0, 16, bar);
+                bulk_load(sdst + 16, s0 + P, 16, bar);
             }
         }
+        __syncwarp();
         ++issued;
         if (++slot == uint32_t(G::kSlots)) {
             slot = 0;
             phase ^= 1;
         }
-        return __all_sync(0xffffffffu, ok);
+        return true;
     }
 };
 

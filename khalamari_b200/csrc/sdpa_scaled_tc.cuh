@@ -7,19 +7,23 @@
 // Codes become 16-bit operands of the Q/output type once per step of 64 tokens, in shared memory, with their row's
 // power-of-two scale already applied: int8 and E4M3 codes times 2^e are exact in bf16, and in f16 as far as its range goes
 // (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). At head_dim 128 two Q tiles of
-// the same sequence and KV head share every converted step (at 256 tensor memory holds the output of one). A probability is rounded to the Q/output type: in bf16 that is off by
-// at most 2^-8, no more than what the cache rounds off a V element (2^-8 to 2^-7 of the row's largest).
+// the same sequence and KV head share every converted step (at 256 tensor memory holds the output of one). A probability
+// is rounded to the Q/output type: in bf16 that is off by at most 2^-8, no more than what the cache rounds off a V element
+// (2^-8 to 2^-7 of the row's largest).
 //
-// Each tile has two score buffers, so that the scores of step j + 1 are computed while the softmax of step j runs and the
-// softmax warps never wait for the tensor cores in the steady state. (With one buffer of 128 tokens a tile the loop
-// softmax -> P V -> Q K^T -> softmax was a chain of 7,200 cycles a step, 3,300 of them waiting.) What bounds it then is the
-// softmax itself: an exponential for every score is 16 a cycle and SM, 1,024 cycles for 128 x 128 scores, about what the
-// two products of such a block take; and the issue slots, of which the conversion needs about as many as the softmax of
-// one tile - hence the two tiles per conversion.
+// Each tile has two score buffers, so that the scores of step j + 1 are computed while the softmax of step j runs. (With
+// one buffer of 128 tokens a tile the loop softmax -> P V -> Q K^T -> softmax was a chain of 7,200 cycles a step, 3,300 of
+// them waiting.) A step of two tiles then takes 2,400 cycles at head_dim 128: a softmax warp spends 500 on loading and the
+// maximum, 1,050 on the exponentials (the special-function unit's share is 512 a tile, 1,024 for both), 350 waiting for
+// scores; the products of both tiles take 1,200, bound by the operands that they read from shared memory. Copies and
+// conversion have to keep ahead of that, which takes eight conversion warps (a unit of 16 rows takes 650 cycles, nearly all
+// of them latency) and two copy warps (one warp issues a copy and its scale bytes every 660 cycles).
 //
-// Warps: 0-3 softmax and epilogue of tile A (one thread a row), 4-7 of tile B (head_dim 256: conversion), 8-12
-// conversion, 13 and 15 tensor-core issue (one lane, a warp for each tile), 14 task decoding and copies. All waits are bounded (mbar_wait); no named
-// barriers between roles.
+// Four sequences of 2,048 new tokens behind contexts of 2,048 to 12,288 (64 / 8 heads, head_dim 128, bf16, int8): 1,750 us,
+// 810 TFLOP/s. 517 tokens at head_dim 256 (16 / 2 heads, f16, E4M3): 39 us with the reduce.
+//
+// Warps: softmax and epilogue, one thread a row (0-3 tile A, 4-7 tile B), conversion (8), tensor-core issue (one lane, a
+// warp for each tile), task decoding and copies (2). All waits are bounded (mbar_wait); no named barriers between roles.
 #pragma once
 
 #include "scaled_kv.cuh"
@@ -47,13 +51,19 @@ struct ScaledTc {
     // Conversion warps take (chunk, K or V) units in turn. A wait tells a barrier's phases apart by their parity only, and a
     // warp does not wait for every copy, nor do copies land in order; so every slot has two barriers used in turn. Then
     // the phase before the one that a warp waits for belongs to copy r - 2 kRawSlots, which is known to have landed: the
-    // warp's last unit was of copy r - kRawSlots or a later one, that copy landed, hence r - kRawSlots had been issued (in
+    // warp's last unit was of copy r - 4, by the same copy warp; that copy landed, hence r - kRawSlots had been issued (in
     // order), hence r - 2 kRawSlots had left the slot. (Chunks past the end of a task count as copies: the distance between
     // a warp's units is fixed.)
-    static constexpr int kConverters = D == 128 ? 5 : 8;
+    static constexpr int kConverters = 8;
     static constexpr int kRawBars = 2 * kRawSlots;
-    static_assert(kConverters <= 13 - kSoftmaxWarps && kConverters <= 2 * kRawSlots, "conversion warps");
-    static constexpr int kThreads = 16 * 32;
+    static_assert(kConverters == 2 * kChunks && kRawSlots % 4 == 0, "a unit of every step, slots of one copy warp");
+    static constexpr int kIssueWarp = kSoftmaxWarps + kConverters, kCopyWarp = kIssueWarp + 2;
+    static constexpr int kThreads = (kIssueWarp + 4) * 32;
+    // The softmax warps need more registers than the launch gives a thread (96 of 640, 128 of 512), the others fewer.
+    static constexpr int kSoftmaxRegisters = D == 128 ? 144 : 200, kOtherRegisters = D == 128 ? 64 : 104;
+    static constexpr int kRescale = D == 128 ? 16 : 64;          // columns of O scaled at a time, as registers allow
+    static_assert(kSoftmaxWarps * kSoftmaxRegisters + (kThreads / 32 - kSoftmaxWarps) * kOtherRegisters <=
+                      kThreads / 32 * (65536 / kThreads / 8 * 8), "registers of the launch");
     static constexpr int kSmemBytes = kTiles * kQBytes + 2 * kStages * kOperandBytes + kRawSlots * (kRawBytes + 32) + 1024 + 1024;
     static_assert(kSmemBytes <= 227 * 1024, "shared memory");
 };
@@ -69,11 +79,6 @@ struct ScaledTcTask {
     uint32_t tok_begin[2], num_toks[2], kv_begin[2], kv_end[2];
 };
 
-// A wait of a whole warp: the same answer in every lane.
-__device__ __forceinline__ bool mbar_wait_warp(uint32_t bar, uint32_t parity, volatile uint32_t* abort_flag, const MapParams& p) {
-    return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, p));
-}
-
 // Two f32 operations in one instruction.
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 r;
@@ -86,14 +91,6 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     asm("{ .reg .b64 a, b, d; mov.b64 a, {%2, %3}; mov.b64 b, {%4, %5}; add.rn.f32x2 d, a, b; mov.b64 {%0, %1}, d; }"
         : "=f"(r.x), "=f"(r.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
     return r;
-}
-
-// One lane of a converged warp, the same one every time. Tensor-core instructions issued under it need no handling of
-// operands that differ between lanes, which under `lane == 0` costs each of them about a hundred cycles.
-__device__ __forceinline__ bool elect_one() {
-    uint32_t elected;
-    asm volatile("{ .reg .pred p; elect.sync _|p, 0xffffffff; selp.u32 %0, 1, 0, p; }" : "=r"(elected));
-    return elected != 0;
 }
 
 template <typename T, int CODE, int D>
@@ -123,7 +120,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     uint32_t* const tmem_slot = const_cast<uint32_t*>(abort_flag) + 1;
     static_assert(sizeof(ScaledTcTask) * 2 + kBars * 8 + 16 <= 1024, "small shared memory");
 
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    // (values from a shuffle are known to be the same in a whole warp: what is computed from them stays in uniform registers,
+    // where the tensor-core instructions and copies take their operands)
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     if (tid == 0) {
         for (int i = 0; i < G::kRawSlots; ++i) {
             mbar_init(raw_empty + 8 * i, 2);  // its K and its V have been converted
@@ -143,7 +142,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             mbar_init(o_free + 8 * i, 4);
             mbar_init(pv_done + 8 * i, 1);
             mbar_init(task_full + 8 * i, 1);
-            mbar_init(task_empty + 8 * i, G::kSoftmaxWarps + G::kConverters + G::kTiles);
+            mbar_init(task_empty + 8 * i, G::kSoftmaxWarps + G::kConverters + G::kTiles + 1);  // (1: the second copy warp)
         }
         mbar_init(drain, G::kTiles);
         *abort_flag = 0;
@@ -156,13 +155,15 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
     tmem_fence_before();
     __syncthreads();
     tmem_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
     const uint32_t tmem_s = tmem, tmem_o = tmem + 256;  // + 128 * tile (+ 64 * buffer); P over the first half of its S
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const ActiveCounts a = resolve_active(p);
 
     if (warp >= uint32_t(G::kSoftmaxWarps)) {
-        if (warp == 14) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(G::kOtherRegisters));
+        if (warp >= uint32_t(G::kCopyWarp)) {
+            const uint32_t which = warp - G::kCopyWarp;
             // ------------------------------ tasks and copies --------------------------------------------------------
             // Tasks are pairs of neighbouring templates, dealt round robin KV head by KV head, so that at any moment the
             // CTAs read the same K/V rows through L2; within a head from the last template to the first, so that the
@@ -174,7 +175,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             const uint64_t total = uint64_t(pairs) * cells;
             const uint32_t page_shift = 31 - __clz(int(p.tokens_per_page));
             const uint64_t policy = l2_evict_first_policy();
-            uint32_t published = 0, issued = 0;
+            uint32_t published = 0;          // tasks
+            uint32_t copied = 0, next = 2 * which;  // running numbers of chunks: of tasks done, of this warp's next pair
             bool ok = true;
             // Two neighbouring templates at once, a half warp each: is there a tile to work on, and for which request.
             auto decode = [&](uint32_t tmpl0, ScaledTcTask& task, uint32_t& slot0, uint32_t& slot1) -> uint32_t {
@@ -284,27 +286,37 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 task.first = task.begin / 16 * 16;
                 task.steps = task.end > task.first ? (task.end - task.first + G::kStep - 1) / G::kStep : 0;
             };
-            next_task();
+            // Both copy warps run this: each copies every other pair of chunks, and the first one decodes and publishes.
+            if (which == 0) next_task();
             while (ok) {
                 const uint32_t ts = published & 1;
-                ok = mbar_wait_warp(task_empty + 8 * ts, ((published >> 1) & 1) ^ 1, abort_flag, p);
+                const uint32_t bar = which == 0 ? task_empty + 8 * ts : task_full + 8 * ts;
+                ok = mbar_wait_warp(bar, ((published >> 1) & 1) ^ (which == 0 ? 1 : 0), abort_flag, p);
                 if (!ok) break;
-                if (lane == 0) {
-                    tasks[ts] = task;
-                    mbar_arrive(task_full + 8 * ts);
+                if (which == 0) {
+                    if (lane == 0) {
+                        tasks[ts] = task;
+                        mbar_arrive(task_full + 8 * ts);
+                    }
+                    __syncwarp();
                 }
                 ++published;
-                if (task.done) break;
                 // what streaming needs; the next task is decoded on the way, once the ring is full
-                const uint32_t begin = task.begin, end = task.end, first = task.first, kv_head = task.kv_head;
-                const uint64_t table = (uint64_t(task.req_slot) * p.num_gqa_layers + p.layer_index) * p.pages_per_request_layer;
+                const ScaledTcTask& now = tasks[ts];
+                if (__shfl_sync(0xffffffffu, now.done, 0)) break;
+                const uint32_t begin = __shfl_sync(0xffffffffu, now.begin, 0), end = __shfl_sync(0xffffffffu, now.end, 0);
+                const uint32_t first = __shfl_sync(0xffffffffu, now.first, 0), kv_head = __shfl_sync(0xffffffffu, now.kv_head, 0);
+                const uint32_t req_slot = __shfl_sync(0xffffffffu, now.req_slot, 0);
+                const uint32_t chunks = __shfl_sync(0xffffffffu, now.steps, 0) * G::kChunks;
+                if (which == 1 && lane == 0) mbar_arrive(task_empty + 8 * ts);
+                const uint64_t table = (uint64_t(req_slot) * p.num_gqa_layers + p.layer_index) * p.pages_per_request_layer;
                 const uint64_t scales = uint64_t((p.num_kv_heads * 2) << page_shift) * D + ((kv_head * 2) << page_shift);
-                const uint32_t slots = end > first ? (end - first + 15) / 16 : 0, chunks = task.steps * G::kChunks;
+                const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
                 uint32_t page0 = 0, page1 = 0;
-                if (slots == 0) next_task();
-                for (uint32_t x = 0; x < chunks && ok; ++x) {
-                    if ((x & 31) == 0 && x + lane < slots) {
-                        const uint32_t token = first + (x + lane) * 16;
+                if (which == 0 && slots == 0) next_task();
+                for (uint32_t x = 2 * which; x < chunks; x += 4) {
+                    if ((x & 31) == 2 * which && (x & ~31u) + lane < slots) {
+                        const uint32_t token = first + ((x & ~31u) + lane) * 16;
                         // (the first half may lie before everything that is visible, the second behind it)
                         const bool low = token + 8 > begin || token + 8 >= end;
                         page0 = p.page_ids[table + ((low ? token : token + 8) >> page_shift)];
@@ -315,49 +327,63 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                             if (page1 >= p.pool_pages) page1 = 0;
                         }
                     }
-                    const uint32_t first_page = __shfl_sync(0xffffffffu, page0, int(x & 31)), second_page = __shfl_sync(0xffffffffu, page1, int(x & 31));
-                    const uint32_t slot = issued % G::kRawSlots, phase = (issued / G::kRawSlots) & 1;
-                    if (lane == 0) {
-                        ok = mbar_wait(raw_empty + 8 * slot, phase ^ 1, abort_flag, p);
-                        const uint32_t bar = raw_full + 8 * (issued % G::kRawBars);
-                        if (ok && x >= slots) mbar_arrive(bar);  // the last step's chunks past the end: nothing to copy
-                        if (ok && x < slots) {
-                            const uint32_t dst = smem_addr(raw_ring) + slot * G::kRawBytes;
-                            const uint32_t sdst = smem_addr(raw_scales) + slot * 32;
-                            const uint32_t in_page = (first + x * 16) & (p.tokens_per_page - 1);  // (8-token pages: 0)
-                            const int32_t page_row = int32_t((kv_head << page_shift) + in_page);
-                            const uint8_t* const s0 = p.kv_pages + uint64_t(first_page) * p.page_bytes + scales + in_page;
-                            mbar_arrive_expect_tx(bar, G::kRawBytes + 32);
-                            tma_load_5d(dst, &kv_map, page_row, int32_t(first_page), bar, policy);
-                            if (page_shift == 3) {
-                                tma_load_5d(dst + G::kRawBytes / 2, &kv_map, page_row, int32_t(second_page), bar, policy);
-                                bulk_load(sdst, s0, 16, bar);
-                                bulk_load(sdst + 16, p.kv_pages + uint64_t(second_page) * p.page_bytes + scales, 16, bar);
-                            } else if (page_shift == 4) {
-                                bulk_load(sdst, s0, 32, bar);
-                            } else {  // half of a 32-token page: its K and its V bytes
-                                bulk_load(sdst, s0, 16, bar);
-                                bulk_load(sdst + 16, s0 + p.tokens_per_page, 16, bar);
+                    uint32_t first_page[2], second_page[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        first_page[i] = __shfl_sync(0xffffffffu, page0, int((x + i) & 31));
+                        second_page[i] = __shfl_sync(0xffffffffu, page1, int((x + i) & 31));
+                    }
+                    const uint32_t number = copied + x, slot = number % G::kRawSlots, phase = (number / G::kRawSlots) & 1;
+                    const uint32_t bar0 = raw_full + 8 * (number % G::kRawBars);
+                    ok = __all_sync(0xffffffffu, mbar_wait(raw_empty + 8 * slot, phase ^ 1, abort_flag, p) &&
+                                                     mbar_wait(raw_empty + 8 * slot + 8, phase ^ 1, abort_flag, p));
+                    if (!ok) break;
+                    if (elect_one()) {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t bar = bar0 + 8 * i;
+                            if (x + i < slots) {
+                                const uint32_t dst = smem_addr(raw_ring) + (slot + i) * G::kRawBytes, sdst = smem_addr(raw_scales) + (slot + i) * 32;
+                                const uint32_t in_page = (first + (x + i) * 16) & (p.tokens_per_page - 1);  // (8-token pages: 0)
+                                const int32_t page_row = int32_t((kv_head << page_shift) + in_page);
+                                const uint8_t* const s0 = p.kv_pages + uint64_t(first_page[i]) * p.page_bytes + scales + in_page;
+                                mbar_arrive_expect_tx(bar, G::kRawBytes + 32);
+                                tma_load_5d(dst, &kv_map, page_row, int32_t(first_page[i]), bar, policy);
+                                if (page_shift == 3) {
+                                    tma_load_5d(dst + G::kRawBytes / 2, &kv_map, page_row, int32_t(second_page[i]), bar, policy);
+                                    bulk_load(sdst, s0, 16, bar);
+                                    bulk_load(sdst + 16, p.kv_pages + uint64_t(second_page[i]) * p.page_bytes + scales, 16, bar);
+                                } else if (page_shift == 4) {
+                                    bulk_load(sdst, s0, 32, bar);
+                                } else {  // half of a 32-token page: its K and its V bytes
+                                    bulk_load(sdst, s0, 16, bar);
+                                    bulk_load(sdst + 16, s0 + p.tokens_per_page, 16, bar);
+                                }
+                            } else {
+                                mbar_arrive(bar);  // the last step's chunks past the end: nothing to copy
                             }
                         }
                     }
-                    ++issued;
-                    ok = __all_sync(0xffffffffu, ok);
-                    if (x == min(slots, uint32_t(G::kRawSlots)) - 1) next_task();
+                    __syncwarp();
+                    next = number + 4;
+                    if (which == 0 && x == ((min(slots, uint32_t(G::kRawSlots)) - 1) & ~3u)) next_task();
                 }
+                copied += chunks;
             }
             if (*abort_flag && lane == 0) {
                 // copies already issued may still be landing
-                for (uint32_t back = 0; back < uint32_t(G::kRawSlots) && back < issued; ++back) {
-                    const uint32_t c = issued - 1 - back;
-                    for (uint32_t i = 0; i < p.wait_limit; ++i) {
-                        if (mbar_try_wait(raw_full + 8 * (c % G::kRawBars), (c / G::kRawBars) & 1)) break;
+                for (uint32_t c = next; c >= 4 && c + G::kRawSlots > next;) {
+                    c -= 4;
+                    for (uint32_t n = c; n < c + 2; ++n) {
+                        for (uint32_t i = 0; i < p.wait_limit; ++i) {
+                            if (mbar_try_wait(raw_full + 8 * (n % G::kRawBars), (n / G::kRawBars) & 1)) break;
+                        }
                     }
                 }
             }
-        } else if (warp >= 13) {
+        } else if (warp >= uint32_t(G::kIssueWarp)) {
             // ------------------------------ tensor-core issue: a warp for each tile, one lane issues ------------------
-            const uint32_t tile = warp == 15 ? 1 : 0;
+            const uint32_t tile = warp - G::kIssueWarp;
             if (tile < uint32_t(G::kTiles)) {
                 constexpr uint32_t kFormat = umma_format<T>();
                 constexpr uint32_t idesc = (1u << 4) | (kFormat << 7) | (kFormat << 10) | ((128u >> 4) << 24);
@@ -394,9 +420,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 for (uint32_t taken = 0; ok; ++taken) {
                     const uint32_t ts = taken & 1;
                     if (!mbar_wait_warp(task_full + 8 * ts, (taken >> 1) & 1, abort_flag, p)) break;
-                    if (tasks[ts].done) break;
-                    const uint32_t steps = tasks[ts].steps;
-                    const bool here = tile == 0 || tasks[ts].active_b != 0;
+                    if (__shfl_sync(0xffffffffu, tasks[ts].done, 0)) break;
+                    const uint32_t steps = __shfl_sync(0xffffffffu, tasks[ts].steps, 0);
+                    const bool here = tile == 0 || __shfl_sync(0xffffffffu, tasks[ts].active_b, 0) != 0;
                     __syncwarp();
                     if (lane == 0) mbar_arrive(task_empty + 8 * ts);
                     if (!here) {
@@ -454,7 +480,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     if (mbar_try_wait(drain, 0)) break;
                 }
             }
-        } else if (warp < uint32_t(G::kSoftmaxWarps + G::kConverters)) {
+        } else {
             // ------------------------------ conversion ---------------------------------------------------------------
             // A warp takes every kConverters-th unit: the K or the V rows of a 16-token chunk. Eight consecutive lanes take the
             // lower four 16-byte pieces of one row and the upper four of its neighbour: that makes their loads, and both
@@ -491,41 +517,50 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     const uint8_t* const scales = raw_scales + slot * 32 + row4;
                     const uint32_t token = first + x * 16;
                     const bool whole = there && token >= begin && token + 16 <= end;
-                    ok = ok && mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
+                    uint4 words[G::kLines][4];
+                    uint32_t b[4];
                     if (!ok) break;
-                    uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
 #pragma unroll
-                    for (int line = 0; line < G::kLines; ++line) {
-                        uint4 words[4];
-                        uint32_t b[4];
+                    for (int i = 0; i < 4; ++i) {
+                        b[i] = scales[plane * scale_plane + (i >> 1) * scale_half + (i & 1) * 4];
+#pragma unroll
+                        for (int line = 0; line < G::kLines; ++line) {
+                            const uint32_t at = (plane * G::kLines + line) * line_stride + (i >> 1) * half_stride + (i & 1) * 512;
+                            words[line][i] = *reinterpret_cast<const uint4*>(source + at + (in_lane ^ ((i & 1) * 64)));
+                        }
+                    }
+                    // the slot takes its next copy while this one is converted
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(raw_empty + 8 * slot);
+                    ok = mbar_wait_warp((plane == 0 ? k_empty : v_empty) + 8 * stage, phase ^ 1, abort_flag, p);
+                    if (!ok) break;
+                    if (!whole) {  // rows that nothing sees may hold anything
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t at = (plane * G::kLines + line) * line_stride + (i >> 1) * half_stride + (i & 1) * 512;
-                            words[i] = *reinterpret_cast<const uint4*>(source + at + (in_lane ^ ((i & 1) * 64)));
-                            b[i] = scales[plane * scale_plane + (i >> 1) * scale_half + (i & 1) * 4];
-                        }
-                        if (!whole) {  // rows that nothing sees may hold anything
+                            const uint32_t t = token + 4 * i + row4;
+                            if (!there || t < begin || t >= end) {
+                                b[i] = 0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) {
-                                const uint32_t t = token + 4 * i + row4;
-                                if (!there || t < begin || t >= end) {
-                                    words[i] = make_uint4(0, 0, 0, 0);
-                                    b[i] = 0;
-                                }
+                                for (int line = 0; line < G::kLines; ++line) words[line][i] = make_uint4(0, 0, 0, 0);
                             }
                         }
-                        bool saturate = false;
-                        if constexpr (std::is_same<T, __half>::value) {
-                            bool large = false;
+                    }
+                    uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
+                    bool saturate = false;
+                    if constexpr (std::is_same<T, __half>::value) {
+                        bool large = false;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i) large = large || (b[i] >= first_large_byte<T>() && b[i] < 255);
-                            saturate = __any_sync(0xffffffffu, large);
-                        }
+                        for (int i = 0; i < 4; ++i) large = large || (b[i] >= first_large_byte<T>() && b[i] < 255);
+                        saturate = __any_sync(0xffffffffu, large);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t one, two;
-                            scaled_factors<T>(b[i], plane == 1, one, two);
-                            const uint32_t raw_words[4] = {words[i].x, words[i].y, words[i].z, words[i].w};
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t one, two;
+                        scaled_factors<T>(b[i], plane == 1, one, two);
+#pragma unroll
+                        for (int line = 0; line < G::kLines; ++line) {
+                            const uint4 w4 = words[line][i];
+                            const uint32_t raw_words[4] = {w4.x, w4.y, w4.z, w4.w};
                             uint32_t r[8];
 #pragma unroll
                             for (int w = 0; w < 4; ++w) decode4<T, CODE>(raw_words[w], one, two, r[2 * w], r[2 * w + 1]);
@@ -542,10 +577,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                     __syncwarp();
-                    if (lane == 0) {
-                        mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
-                        mbar_arrive(raw_empty + 8 * slot);
-                    }
+                    if (lane == 0) mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
                 }
                 unit += units;
                 step += steps;
@@ -553,6 +585,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
         }
     } else {
         // ------------------------------ softmax and epilogue of one tile: a thread per row ----------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(G::kSoftmaxRegisters));
         const uint32_t tile = warp / 4, quad = warp % 4;
         const uint32_t row = quad * 32 + lane;
         const uint32_t lane_base = (quad * 32) << 16;
@@ -632,13 +665,15 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         if (!ok) break;
                         tmem_fence_after();
 #pragma unroll
-                        for (int c = 0; c < D; c += 16) {
-                            uint32_t o[16];
-                            tmem_ld16(o, o_at + c);
+                        for (int c = 0; c < D; c += G::kRescale) {
+                            uint32_t o[G::kRescale];
+#pragma unroll
+                            for (int i = 0; i < G::kRescale; i += 16) tmem_ld16(*reinterpret_cast<uint32_t(*)[16]>(&o[i]), o_at + c + i);
                             tmem_ld_wait();
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
-                            tmem_st16(o_at + c, o);
+                            for (int i = 0; i < G::kRescale; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+#pragma unroll
+                            for (int i = 0; i < G::kRescale; i += 16) tmem_st16(o_at + c + i, *reinterpret_cast<uint32_t(*)[16]>(&o[i]));
                         }
                         tmem_st_wait();
                     }
