@@ -3,7 +3,8 @@
 // Compiles the CUDA sources of libkhcuda_gqa for sm_100a with nvcc and links the crate against the result: the
 // same single nvcc command `khalamari_b200/build.py` runs for the Python harness.
 //
-//   KHCUDA_GQA_CSRC   directory holding host_sdpa.cpp, sdpa_api.cu, sdpa_fp8.cu, kv_page_write.cu, bidi_block_sdpa.cu and their
+//   KHCUDA_GQA_CSRC   directory holding host_sdpa.cpp, sdpa_api.cu, sdpa_fp8.cu, sdpa_scaled.cu, kv_page_write.cu,
+//                     kv_page_read.cu, bidi_block_sdpa.cu, peer_exchange.cu and their
 //                     headers (default: ../khalamari_b200/csrc relative to this crate)
 //   KHCUDA_GQA_DIR    use a prebuilt libkhcuda_gqa.so from this directory instead of compiling
 //   NVCC              nvcc binary (default: nvcc on PATH, else /usr/local/cuda/bin/nvcc)
@@ -11,9 +12,11 @@ use std::env;
 use std::path::{Path, PathBuf};
 use std::process::Command;
 
-const SOURCES: [&str; 6] =
-    ["host_sdpa.cpp", "sdpa_api.cu", "sdpa_fp8.cu", "kv_page_write.cu", "bidi_block_sdpa.cu", "peer_exchange.cu"];
-const HEADERS: [&str; 7] = ["common.h", "cuda_objects.h", "host_sdpa.h", "map_instance.h", "sdpa_map.cuh", "sdpa_tc.cuh", "sdpa_tm.cuh"];
+const SOURCES: [&str; 8] =
+    ["host_sdpa.cpp", "sdpa_api.cu", "sdpa_fp8.cu", "sdpa_scaled.cu", "kv_page_write.cu", "kv_page_read.cu", "bidi_block_sdpa.cu",
+     "peer_exchange.cu"];
+const HEADERS: [&str; 10] = ["common.h", "cuda_objects.h", "host_sdpa.h", "map_instance.h", "sdpa_map.cuh", "sdpa_tc.cuh", "sdpa_tm.cuh",
+                             "sdpa_scaled.cuh", "sdpa_scaled_tc.cuh", "scaled_kv.cuh"];
 
 fn main() {
     println!("cargo:rerun-if-env-changed=KHCUDA_GQA_DIR");

@@ -32,7 +32,8 @@ impl PageTableLayout {
 }
 
 /// `kv_page_write::Config` (`kv_page_write.rs:62-68`) plus the stored element type: `Dtype::Fp8E4M3FN` is the
-/// reference's store; `kv_dtype == dtype` keeps the source bits (the page format the 16-bit kernels read).
+/// reference's store; `kv_dtype == dtype` keeps the source bits (the page format the 16-bit kernels read); the scaled
+/// types quantise each row under a power-of-two scale of its own.
 #[derive(Clone, Copy, Debug, Eq, PartialEq)]
 pub struct Config {
     pub num_kv_heads: u32,

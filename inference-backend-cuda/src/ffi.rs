@@ -20,6 +20,8 @@ pub const KH_DTYPE_FLOAT16: u32 = 9;
 pub const KH_DTYPE_FLOAT32: u32 = 10;
 pub const KH_DTYPE_BFLOAT16: u32 = 12;
 pub const KH_DTYPE_FP8_E4M3FN: u32 = 100;
+pub const KH_DTYPE_INT8_SCALED: u32 = 101;
+pub const KH_DTYPE_FP8_E4M3FN_SCALED: u32 = 102;
 
 pub const KH_MAP_SLICED_KV: u32 = 0;
 pub const KH_MAP_Q_TOKENS_PER_HEAD: u32 = 1;
@@ -28,6 +30,7 @@ pub const KH_MAP_Q_TOKENS_AND_HEADS: u32 = 3;
 
 pub const KH_POLICY_REFERENCE: u32 = 0;
 pub const KH_POLICY_B200: u32 = 1;
+pub const KH_POLICY_B200_CHAINED: u32 = 2;
 
 /// Bytes of the partial-state array `kh_sliced_kv_attend_static` works in.
 pub const KH_STATIC_PARTIALS_BYTES: u64 = 32 << 20;
@@ -88,6 +91,12 @@ pub struct KhSlicedQ {
 /// Opaque handle (`kh_kv_page_write`).
 #[repr(C)]
 pub struct KhKvPageWrite {
+    _private: [u8; 0],
+}
+
+/// Opaque handle (`kh_kv_page_read`).
+#[repr(C)]
+pub struct KhKvPageRead {
     _private: [u8; 0],
 }
 
@@ -369,6 +378,24 @@ pub struct KhKvPageWriteShape {
 #[repr(C)]
 #[derive(Clone, Copy, Debug)]
 pub struct KhKvPageWriteBuffers {
+    pub pages: KhBufferRef,
+    pub flat_k: KhBufferRef,
+    pub flat_v: KhBufferRef,
+    pub req_slots: KhBufferRef,
+    pub flat_token_indices: KhBufferRef,
+    pub page_ids: KhBufferRef,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct KhKvPageReadShape {
+    pub num_total_token_reads: u32,
+    pub page_table_layout: KhPageTableLayout,
+}
+
+#[repr(C)]
+#[derive(Clone, Copy, Debug)]
+pub struct KhKvPageReadBuffers {
     pub pages: KhBufferRef,
     pub flat_k: KhBufferRef,
     pub flat_v: KhBufferRef,
@@ -737,6 +764,20 @@ unsafe extern "C" {
         shape: *const KhKvPageWriteShape,
         buffers: *const KhKvPageWriteBuffers,
         num_active_token_writes: u32,
+        page_table_index: u32,
+    ) -> KhStatus;
+    pub fn kh_kv_page_read_create(
+        device: *mut KhDevice,
+        config: *const KhKvPageWriteConfig,
+        out: *mut *mut KhKvPageRead,
+    ) -> KhStatus;
+    pub fn kh_kv_page_read_destroy(compute: *mut KhKvPageRead) -> KhStatus;
+    pub fn kh_kv_page_read_invoke(
+        compute: *mut KhKvPageRead,
+        stream: *mut KhStream,
+        shape: *const KhKvPageReadShape,
+        buffers: *const KhKvPageReadBuffers,
+        num_active_token_reads: u32,
         page_table_index: u32,
     ) -> KhStatus;
     pub fn kh_fp8_e4m3_from_bf16(bf16_bits: u16) -> u8;

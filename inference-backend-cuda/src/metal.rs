@@ -19,6 +19,9 @@ pub enum Dtype {
     Bfloat16 = ffi::KH_DTYPE_BFLOAT16,
     /// KV-cache pages only: the reference's one-byte cache format (`components/gqa/fp8.rs`).
     Fp8E4M3FN = ffi::KH_DTYPE_FP8_E4M3FN,
+    /// KV-cache pages only: one byte an element and a power-of-two scale byte for each token and KV head.
+    Int8Scaled = ffi::KH_DTYPE_INT8_SCALED,
+    Fp8E4M3Scaled = ffi::KH_DTYPE_FP8_E4M3FN_SCALED,
 }
 
 impl Dtype {
@@ -26,8 +29,17 @@ impl Dtype {
         match self {
             Dtype::Float16 | Dtype::Bfloat16 => 2,
             Dtype::Float32 => 4,
-            Dtype::Fp8E4M3FN => 1,
+            Dtype::Fp8E4M3FN | Dtype::Int8Scaled | Dtype::Fp8E4M3Scaled => 1,
         }
+    }
+
+    pub fn is_scaled(self) -> bool {
+        matches!(self, Dtype::Int8Scaled | Dtype::Fp8E4M3Scaled)
+    }
+
+    /// Bytes of one stored K or V row of one token and KV head: scaled pages add the row's scale byte.
+    pub fn kv_row_bytes(self, head_dim: usize) -> usize {
+        head_dim * self.item_size() + usize::from(self.is_scaled())
     }
 }
 

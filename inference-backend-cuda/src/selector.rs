@@ -33,6 +33,8 @@ impl RequestShape {
 pub enum SelectorPolicy {
     Reference,
     B200,
+    /// `B200` with shorter decode slices, for the Map kernels of scaled pages, which merge neighbouring slices.
+    B200Chained,
 }
 
 pub type GQAReplayShape = ffi::KhReplayShape;
@@ -57,6 +59,7 @@ impl Selector {
         let policy = match policy {
             SelectorPolicy::Reference => ffi::KH_POLICY_REFERENCE,
             SelectorPolicy::B200 => ffi::KH_POLICY_B200,
+            SelectorPolicy::B200Chained => ffi::KH_POLICY_B200_CHAINED,
         };
         expect_ok(unsafe { ffi::kh_selector_set_policy(self.raw, policy, sm_count) }, "Selector::set_policy");
     }

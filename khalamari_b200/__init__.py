@@ -14,6 +14,8 @@ module                      reference file
 ``request_page_table``      crates/inference-executor-metal/src/attn/gqa/request_page_table.rs
 ``replay``                  crates/inference-executor-core/src/replay.rs
 ``gqa``                     crates/inference-executor-metal/src/attn/gqa/backend.rs (prepare, record_sdpa)
+``kv_page_write``           crates/inference-backend-metal/src/components/gqa/kv_page_write.rs
+``kv_page_read``            (none: its inverse)
 ``device``                  crates/inference-backend-metal/src/metal/{device,buffer,stream}
 ==========================  =====================================================================
 """

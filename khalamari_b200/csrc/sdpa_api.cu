@@ -455,6 +455,8 @@ static void launch_map(ComputeCommon& c, kh_stream* stream, MapParams& p, kh_buf
         KH_REQUIRE(p.cu == nullptr, "scaled 8-bit pages: the one-launch map + reduce form is not available");
         KH_REQUIRE((reinterpret_cast<uintptr_t>(kv_pages.ptr) & 15) == 0, "kv_pages must be 16-byte aligned");
         KH_REQUIRE((reinterpret_cast<uintptr_t>(q.ptr) & 15) == 0, "q must be 16-byte aligned");
+        KH_REQUIRE((reinterpret_cast<uintptr_t>(p.direct != 0 ? p.out : p.partial_out) & 15) == 0, "%s must be 16-byte aligned",
+                   p.direct != 0 ? "output" : "partial_output");
         KH_REQUIRE(c.page_bytes <= 0x7fffffffu, "scaled 8-bit pages must be smaller than 2 GiB");
         p.q = q.ptr;
         p.kv_pages = static_cast<const uint8_t*>(kv_pages.ptr);
@@ -1580,6 +1582,7 @@ kh_status kh_sliced_kv_attend_static(kh_sliced_kv* compute, kh_stream* stream,
         r.num_partials = num_active_kv_splits;  // the sections of the shared array are sized for exactly these
         r.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         r.active_range_word = 0;
+        r.wide = wide_reduce(config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens, r.head_dim);
         launch_reduce(config.dtype, r, num_active_tokens, stream->stream);
         return KH_OK;
     });

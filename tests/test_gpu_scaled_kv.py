@@ -421,6 +421,48 @@ def test_unaligned_buffers_and_the_one_launch_form_are_refused(device):
         run.record()
 
 
+def test_unaligned_direct_output_is_refused(device):
+    from khalamari_b200 import abi
+    from khalamari_b200.device import Buffer
+    case = make_scaled_case(43, "int8", "bf16", 16, 2, 128, [0], [40])
+    run = ScaledRun(device, case, max_tokens=512)
+    run.plan()
+    if not run.attention.metadata.direct_output():
+        pytest.skip("this batch is not written directly")
+    run.out = Buffer.wrap(device, run.out.ref.ptr + 2, run.out.len_bytes() - 2)
+    with pytest.raises(abi.InvalidArgument, match="output must be 16-byte aligned"):
+        run.record()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("d", [128, 256])
+@pytest.mark.parametrize("hq,q_len", [(16, 1), (32, 1), (16, 2), (32, 3), (64, 1), (32, 40)])
+def test_groups_of_many_heads(device, code, d, hq, q_len):
+    """One KV head for 16 to 64 Q heads: tasks of 16 rows and more, and groups cut into ranges of heads."""
+    case = make_scaled_case(hq + q_len, code, "bf16", hq, 1, d, [700 - q_len, 33], [q_len, q_len])
+    run = ScaledRun(device, case, max_tokens=512)
+    out = run.run()
+    assert_close(out, *reference(case, wide=run.wide()))
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("hq,hkv,d,contexts", [(64, 8, 128, [3000, 17, 1024, 640]), (16, 2, 256, [900, 4100, 33])])
+def test_the_shared_array_form_gives_the_same_bits(device, code, hq, hkv, d, contexts):
+    from khalamari_b200 import sliced_kv
+    case = make_scaled_case(91, code, "bf16", hq, hkv, d, [c - 1 for c in contexts], [1] * len(contexts))
+    run = ScaledRun(device, case)
+    expected = run.run()
+    meta = run.attention.metadata
+    shape = meta.replay_shape()
+    compute = run.attention._sliced_kv(shape, meta.variant())
+    run.out.write(0, np.full(run.out_rows * run.row, run.canary, np.uint16))
+    compute.invoke_attend_static(
+        run.stream, sliced_kv.StaticBuffers(run.q, run.pages, meta.req_slots(), run.ids, meta.sdpa_map_task_templates(),
+                                            meta.cu_sdpa_partial_outputs(), run.out),
+        case.layer, shape.num_tokens, shape.num_sdpa_map_task_templates)
+    assert np.array_equal(expected, run.read())
+
+
 @pytest.mark.parametrize("code", CODES)
 def test_append_then_attend_over_several_steps(device, code):
     """The operators together, as a serving loop has them: each step writes the new token's rows and attends; at the
