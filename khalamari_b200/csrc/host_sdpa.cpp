@@ -468,7 +468,13 @@ Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* request
             tiles_total += tiles;
             work += (unsigned __int128)tiles * (requests[r].num_history_tokens + requests[r].num_q_tokens);
         }
-        if (sliced_q && tiles_total * head_groups >= uint64_t(sm_count) * kTasksPerSm) {
+        // The chained kernels' wide tiles (more than 32 rows) are whole from fewer tasks on: at head_dim 128 two
+        // neighbouring tiles share every K/V step at the price of one, which cutting the KV range would give up
+        // (2,048 tokens behind 3,900, 64 / 8 heads: 806 us cut, 437 us whole), and at 256 the partials of cut tiles cost
+        // more than a last round that is half empty (2 x 2,048 tokens behind 4,000, 32 / 4 heads: 1,320 us cut, 894 us whole).
+        const bool wide = chained && variant.max_q_tokens * variant.max_q_heads > 32;
+        const uint32_t whole = !wide ? kTasksPerSm : c.head_dim == 128 ? 1 : 2;
+        if (sliced_q && tiles_total * head_groups >= uint64_t(sm_count) * whole) {
             // enough (Q tile, head group) tasks to fill every SM several times over without cutting the KV range:
             // one task per tile writes the output directly, no partials and no reduce (chunked prefill)
             slice = end;

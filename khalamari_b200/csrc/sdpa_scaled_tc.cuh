@@ -169,8 +169,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             // CTAs read the same K/V rows through L2; within a head from the last template to the first, so that the
             // long rows of a causal batch do not come last.
             const uint32_t cells = p.num_kv_heads * p.head_ranges;
-            // (few tasks: one tile each, on as many SMs)
-            const uint32_t stride = G::kTiles == 2 && uint64_t(a.templates) * cells >= 2 * uint64_t(gridDim.x) ? 2 : 1;
+            // (no more tasks than SMs: one tile each; a pair costs about what a single tile does)
+            const uint32_t stride = G::kTiles == 2 && uint64_t(a.templates) * cells > gridDim.x ? 2 : 1;
             const uint32_t pairs = (a.templates + stride - 1) / stride;
             const uint64_t total = uint64_t(pairs) * cells;
             const uint32_t page_shift = 31 - __clz(int(p.tokens_per_page));

@@ -86,3 +86,22 @@ def test_restated_attention_matches_a_softmax_over_the_decoded_rows(code):
     k, v = case.k[1][:2, 1], case.v[1][:2, 1]
     w = np.exp(k @ q[2, 3] * case.scale)
     assert np.allclose(out[2, 3], w @ v / w.sum(), rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("hq,hkv,d,q_len,history,whole", [
+    (64, 8, 128, 2048, 3900, True),    # 1,024 tasks
+    (64, 8, 128, 256, 3900, False),    # 128 tasks: fewer than SMs
+    (16, 2, 256, 2048, 3900, False),   # 256 tasks, one tile at a time
+    (32, 4, 256, 2048, 3900, True),    # 512 tasks
+])
+def test_the_chained_policy_keeps_wide_tiles_whole_from_fewer_tasks_on(hq, hkv, d, q_len, history, whole):
+    from khalamari_b200.replay import GQAReplayBucketPolicy
+    from khalamari_b200.selector import RequestShape, Selector, SelectorPolicy
+    layout = GQAPageTableLayout(1, 1, 1024, 1)
+    for policy, expected in ((SelectorPolicy.B200Chained, whole), (SelectorPolicy.B200, False)):
+        selector = Selector.for_lookup(SdpaConfig(Dtype.Bfloat16, hq, hkv, d, 16), 4096, layout)
+        selector.set_policy(policy, 148)
+        limits = selector.limits()
+        buckets = GQAReplayBucketPolicy(limits.max_tokens, limits.max_map_task_templates)
+        selection = selector.select([RequestShape(history, q_len)], buckets, q_len)
+        assert selection.direct_output() == expected
