@@ -28,9 +28,10 @@ static MapInstance make_tc_instance() {
     return MapInstance{sdpa_scaled_tc_kernel<T, CODE, D>, G::kThreads, G::kSmemBytes, G::kStep, 16, G::kRawSlots, 0};
 }
 
-// Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM. Tasks wider than the widest
-// instance are worked on in blocks of rows, which read the KV range again (from L2). `paired`: the KV heads can be taken
-// two at a time.
+// Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM; wider tasks go to tcgen05, whose
+// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 506 us here, 856 us there; a quarter of
+// the Q rows of a tile is where it begins to pay). `paired`: the KV heads can be taken two at a time (64 decode sequences:
+// 145 us, one at a time 150 us).
 template <typename T, int CODE, int D>
 static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {
     if constexpr (D == 128) {
