@@ -17,7 +17,6 @@ struct MapInstance {
     int stage_tokens;
     int box_rows;
     int stages;
-    int rows_per_block = 0;  // scaled pages: Q rows of a task that one work item takes; 0: all of them
 };
 
 // Warp-level instance for K/V pages of FP8 E4M3FN elements (sdpa_fp8.cu; compiled apart from the 16-bit instances

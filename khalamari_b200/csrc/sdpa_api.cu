@@ -490,10 +490,7 @@ static void launch_map(ComputeCommon& c, kh_stream* stream, MapParams& p, kh_buf
     }
 #endif
     if (num_templates == 0) return;
-    uint64_t tasks = uint64_t(num_templates) * c.num_kv_heads * p.head_ranges;
-    if (c.instance.rows_per_block != 0) {
-        tasks *= div_ceil(p.max_q_tokens * p.heads_per_task, uint32_t(c.instance.rows_per_block));
-    }
+    const uint64_t tasks = uint64_t(num_templates) * c.num_kv_heads * p.head_ranges;
     KH_REQUIRE(tasks <= 0xffffffffull, "GQA SDPA map task count must fit u32");
     const uint32_t grid = static_cast<uint32_t>(std::min<uint64_t>(tasks, uint64_t(c.device->sm_count)));
     const MapInstance& instance = p.cu != nullptr ? c.fused_instance : c.instance;

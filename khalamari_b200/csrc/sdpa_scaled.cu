@@ -13,24 +13,23 @@ template <typename T, int CODE, int D, int NQ, int W, int HP, int NT>
 static MapInstance make_stream_instance() {
     using G = ScaledGeometry<D, NQ, W, HP, true>;
     return MapInstance{sdpa_scaled_stream_kernel<T, CODE, D, NQ, W, HP, NT>, G::kThreads, G::kSmemBytes, G::kTileTokens, HP * 16,
-                       G::kSlots, G::kRows};
+                       G::kSlots};
 }
 
 template <typename T, int CODE, int D, int NQ, int W>
 static MapInstance make_chain_instance() {
     using G = ScaledGeometry<D, NQ, W, 1, false>;
-    return MapInstance{sdpa_scaled_chain_kernel<T, CODE, D, NQ, W>, G::kThreads, G::kSmemBytes, G::kTileTokens, 16, G::kSlots, G::kRows};
+    return MapInstance{sdpa_scaled_chain_kernel<T, CODE, D, NQ, W>, G::kThreads, G::kSmemBytes, G::kTileTokens, 16, G::kSlots};
 }
 
 template <typename T, int CODE, int D>
 static MapInstance make_tc_instance() {
     using G = ScaledTc<D>;
-    return MapInstance{sdpa_scaled_tc_kernel<T, CODE, D>, G::kThreads, G::kSmemBytes, G::kStep, 16, G::kRawSlots, 0};
+    return MapInstance{sdpa_scaled_tc_kernel<T, CODE, D>, G::kThreads, G::kSmemBytes, G::kStep, 16, G::kRawSlots};
 }
 
 // Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM; wider tasks go to tcgen05, whose
-// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 506 us here, 856 us there; a quarter of
-// the Q rows of a tile is where it begins to pay). `paired`: the KV heads can be taken two at a time (64 decode sequences:
+// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 496 us here, 856 us there). `paired`: the KV heads can be taken two at a time (64 decode sequences:
 // 145 us, one at a time 150 us).
 template <typename T, int CODE, int D>
 static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {

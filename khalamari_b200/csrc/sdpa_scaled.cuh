@@ -1,4 +1,4 @@
-// Map / direct attention kernel over scaled 8-bit pages (scaled_kv.cuh), for tasks of any number of Q rows.
+// Map / direct attention kernels over scaled 8-bit pages (scaled_kv.cuh), for tasks of up to 32 Q rows.
 //
 //   s_t = scale * 2^eK_t * (q . cK_t)      p_t = exp(s_t - m)      out = sum_t p_t 2^eV_t cV_t / sum_t p_t
 //
@@ -22,8 +22,8 @@
 // index pairs (2t, 2t + 1) and (2t + 8, 2t + 9), with Q read in the same order; and 16-byte column g of V rows 2t,
 // 2t + 1, 2t + 8, 2t + 9, which are the fragment's tokens. Under the swizzle both patterns touch every bank once.
 //
-// Work is divided in two ways. In both a CTA gets one contiguous run of work items (template x KV head x Q-head range
-// x block of Q rows; slices of the same rows, a chain, are neighbours), balanced by KV tokens: the run may begin and
+// Work is divided in two ways. In both a CTA gets one contiguous run of work items (template x KV head x Q-head range;
+// slices of the same rows, a chain, are neighbours), balanced by KV tokens: the run may begin and
 // end inside a template (see scaled_cut).
 //  - sdpa_scaled_stream_kernel: the run's tiles are cut into one contiguous share per warp, whatever items they belong
 //    to, and a warp's copies run on across items. A warp that holds all tiles of a chain publishes it by itself; a
@@ -36,7 +36,7 @@
 // heads, 604 MB of codes and scales), the step takes 138-140 us with int8 codes (4.3 TB/s) and 123-127 us with E4M3 (4.8 TB/s),
 // its reduce included: 440 warp instructions per 16-token int8 tile and head, which 12 warps do not hide altogether. 16
 // warps with two slots each took 148 us, 8 warps 160. At head_dim 256, 24 rows (32 sequences of four verify tokens, 24 / 4
-// heads, 1.35 GB): 506 us, 2.7 TB/s; 192 accumulator registers a thread leave two warps a scheduler, which wait for fixed
+// heads, 1.35 GB): 496 us, 2.7 TB/s; 192 accumulator registers a thread leave two warps a scheduler, which wait for fixed
 // latencies. One sequence of 524,288 tokens (16 / 2 heads, 256): 119 us, 4.5 TB/s.
 #pragma once
 
@@ -83,13 +83,13 @@ struct ScaledGeometry {
     static_assert(kParkBytes % 16 == 0 && kQBytes % 16 == 0 && kBigBytes % 1024 == 0, "alignment");
 };
 
-// A work item: one map task template (or a part of one) x KV head x Q-head range x block of kRows Q rows.
+// A work item: one map task template (or a part of one) x KV head x Q-head range; at most kRows Q rows.
 struct ScaledItem {
     uint32_t tmpl, cell;         // cell = KV head x Q-head range; with HP = 2 the first of two
     uint32_t range;              // Q range index: items of equal range and cell are slices of the same rows
-    uint32_t tok_begin, num_toks, row_begin;
-    uint32_t kv_begin, kv_end;   // clipped to what some row of the block sees, and to the CTA's part of the template
-    uint32_t all_begin, all_end; // tokens that every row of the block sees
+    uint32_t tok_begin, num_toks;
+    uint32_t kv_begin, kv_end;   // clipped to what some row sees, and to the CTA's part of the template
+    uint32_t all_begin, all_end; // tokens that every row sees
     uint32_t req_slot;
     uint32_t active;
     uint32_t chain;              // index (in the pass) of the chain's first item
@@ -97,11 +97,11 @@ struct ScaledItem {
     uint32_t slot;               // template index whose partial the chain's part in this CTA is published as, and the
     uint32_t empties;            // number of template indices behind it that are published as empty
 };
-static_assert(sizeof(ScaledItem) == 64, "item size");
+static_assert(sizeof(ScaledItem) <= 64, "item size");
 
 // Q rows of an item, for the lanes that stage, mask and publish them.
 struct ScaledRows {
-    uint32_t head_begin, num_heads, tok_begin, num_toks, row_begin, heads_per_task;
+    uint32_t head_begin, num_heads, tok_begin, num_toks, heads_per_task;
 
     __device__ __forceinline__ ScaledRows(const MapParams& p, const ScaledItem& it, uint32_t pair = 0) {
         const uint32_t cell = it.cell + pair;
@@ -110,13 +110,12 @@ struct ScaledRows {
         num_heads = min(p.heads_per_task, p.group - skipped);
         tok_begin = it.tok_begin;
         num_toks = it.num_toks;
-        row_begin = it.row_begin;
         heads_per_task = p.heads_per_task;
     }
-    __device__ __forceinline__ uint32_t token(uint32_t row) const { return (row_begin + row) / heads_per_task; }  // of the range
-    __device__ __forceinline__ uint32_t head(uint32_t row) const { return head_begin + (row_begin + row) % heads_per_task; }
+    __device__ __forceinline__ uint32_t token(uint32_t row) const { return row / heads_per_task; }  // of the range
+    __device__ __forceinline__ uint32_t head(uint32_t row) const { return head_begin + row % heads_per_task; }
     __device__ __forceinline__ bool valid(uint32_t row) const {
-        return token(row) < num_toks && (row_begin + row) % heads_per_task < num_heads;
+        return token(row) < num_toks && row % heads_per_task < num_heads;
     }
 };
 
@@ -241,19 +240,15 @@ struct ScaledRun {
 
 // Item `index` of a run, cell-major, with the early-return rules of decode_task (sdpa_map.cuh).
 template <int HP>
-__device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const ActiveCounts& a, const ScaledRun& run, uint32_t index,
-                                                  uint32_t rows_per_block, uint32_t row_blocks) {
+__device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const ActiveCounts& a, const ScaledRun& run, uint32_t index) {
     ScaledItem it;
     it.active = 0;
     it.kv_begin = it.kv_end = it.all_begin = it.all_end = 0;
     it.tok_begin = it.num_toks = it.req_slot = 0;
     it.chain = it.length = it.empties = 0;
-    const uint32_t block = index % row_blocks;
-    const uint32_t task = index / row_blocks;
-    it.tmpl = run.begin.tmpl + task;
+    it.tmpl = run.begin.tmpl + index;
     it.slot = it.tmpl;
     it.cell = run.group * HP;
-    it.row_begin = block * rows_per_block;
     it.range = p.templates[uint64_t(it.tmpl) * 3];
     const uint32_t kv_begin = p.templates[uint64_t(it.tmpl) * 3 + 1], kv_end = p.templates[uint64_t(it.tmpl) * 3 + 2];
     if (p.q_ranges == nullptr) {
@@ -267,7 +262,6 @@ __device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const Acti
         it.tok_begin = begin;
         it.num_toks = min(end - begin, p.max_q_tokens);
     }
-    if (it.row_begin >= it.num_toks * p.heads_per_task) return it;  // no Q row in this block
     it.req_slot = p.req_slots[it.tok_begin];
     if (it.req_slot >= p.num_req_slots ||
         (kv_end > kv_begin &&
@@ -276,10 +270,8 @@ __device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const Acti
         return it;
     }
     it.active = 1;
-    const uint32_t first = it.row_begin / p.heads_per_task;
-    const uint32_t last = min((it.row_begin + rows_per_block - 1) / p.heads_per_task, it.num_toks - 1);
     uint32_t any_lo = 0xffffffffu, any_hi = 0, all_lo = 0, all_hi = 0xffffffffu;
-    for (uint32_t tok = first; tok <= last; ++tok) {
+    for (uint32_t tok = 0; tok < it.num_toks; ++tok) {
         uint32_t lo, hi;
         scaled_visible(p, it.tok_begin, tok, kv_begin, kv_end, lo, hi);
         all_lo = max(all_lo, lo);
@@ -290,7 +282,7 @@ __device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const Acti
         }
     }
     // the CTA's part of a template that a cut divides
-    if (task == 0 && run.begin.tile > 0) any_lo = max(any_lo, (kv_begin / 16 + run.begin.tile) * 16);
+    if (index == 0 && run.begin.tile > 0) any_lo = max(any_lo, (kv_begin / 16 + run.begin.tile) * 16);
     if (it.tmpl == run.end.tmpl) any_hi = min(any_hi, (kv_begin / 16 + run.end.tile) * 16);
     if (any_hi > any_lo) {
         it.kv_begin = any_lo;
@@ -305,10 +297,10 @@ __device__ __forceinline__ ScaledItem scaled_item(const MapParams& p, const Acti
 // the items' tiles. A pass ends with the last whole chain that fits it (ONE_CHAIN: with the first); returns its items.
 template <bool ONE_CHAIN>
 __device__ __forceinline__ uint32_t scaled_chains(const MapParams& p, const ScaledRun& run, ScaledItem* items, uint32_t* cum, uint32_t count,
-                                                  bool more, uint32_t row_blocks, uint32_t lane) {
+                                                  bool more, uint32_t lane) {
     // an item continues the one before it when it is another slice of the same Q rows whose state can be carried on
     auto continues = [&](uint32_t i) {
-        return i > 0 && row_blocks == 1 && p.direct == 0 && items[i].active && items[i - 1].active && items[i].range == items[i - 1].range;
+        return i > 0 && p.direct == 0 && items[i].active && items[i - 1].active && items[i].range == items[i - 1].range;
     };
     uint32_t chain = 0, kept = count;
     for (uint32_t base = 0; base < count; base += 32) {
@@ -854,7 +846,7 @@ struct ScaledShare {
 
 // Called by all threads; leaves the share in shared memory (`share`). `big`: the ring, not in use yet.
 template <typename G>
-__device__ __forceinline__ void scaled_share(const MapParams& p, const ActiveCounts& a, uint32_t groups, uint32_t row_blocks,
+__device__ __forceinline__ void scaled_share(const MapParams& p, const ActiveCounts& a, uint32_t groups,
                                              uint32_t* big, uint32_t* scratch, ScaledShare* share) {
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const uint32_t n = a.templates;
@@ -877,7 +869,7 @@ __device__ __forceinline__ void scaled_share(const MapParams& p, const ActiveCou
     } else {
         uint32_t* const prefix = big;
         uint32_t* const ranges = big + n + 1;
-        const bool splittable = row_blocks == 1 && p.direct == 0;
+        const bool splittable = p.direct == 0;
         scaled_prefix<G>(p, n, prefix, ranges, scratch);
         const uint64_t per_group = prefix[n], total = per_group * groups;
         const uint64_t x0 = total * cta / ctas, x1 = total * (cta + 1) / ctas;
@@ -941,7 +933,6 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
     }
     const ActiveCounts a = resolve_active(p);
     const uint32_t groups = p.num_kv_heads * p.head_ranges / HP;
-    const uint32_t row_blocks = (p.max_q_tokens * p.heads_per_task + G::kRows - 1) / G::kRows;
     const ScaledLane<D, HP> at(p.tokens_per_page, pair, lane);
     uint8_t* const my_ring = smem + unit * (S * G::kSlotBytes);
     const uint8_t* const my_scales = scale_ring + unit * (S * G::kScaleBytes);
@@ -953,21 +944,21 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
     uint32_t slot = 0, phase = 0;  // of the next tile to consume
     bool ok = true;
 
-    scaled_share<G>(p, a, groups, row_blocks, reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(park_stats), share);
+    scaled_share<G>(p, a, groups, reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(park_stats), share);
     uint32_t group = share->first, first_item = 0;
     while (group <= share->last) {
         const ScaledRun run = share->run(group, a.templates);
-        const uint32_t run_items = run.templates * row_blocks;
+        const uint32_t run_items = run.templates;
         if (first_item >= run_items) {
             ++group;
             first_item = 0;
             continue;
         }
         const uint32_t seen = min(uint32_t(G::kItems), run_items - first_item);
-        for (uint32_t i = tid; i < seen; i += G::kThreads) items[i] = scaled_item<HP>(p, a, run, first_item + i, G::kRows, row_blocks);
+        for (uint32_t i = tid; i < seen; i += G::kThreads) items[i] = scaled_item<HP>(p, a, run, first_item + i);
         __syncthreads();
         if (warp == 0) {
-            const uint32_t kept = scaled_chains<false>(p, run, items, cum, seen, first_item + seen < run_items, row_blocks, lane);
+            const uint32_t kept = scaled_chains<false>(p, run, items, cum, seen, first_item + seen < run_items, lane);
             if (lane == 0) *pass_items = kept;
         }
         __syncthreads();
@@ -1210,7 +1201,6 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
     }
     const ActiveCounts a = resolve_active(p);
     const uint32_t cells = p.num_kv_heads * p.head_ranges;
-    const uint32_t row_blocks = (p.max_q_tokens * p.heads_per_task + G::kRows - 1) / G::kRows;
     const ScaledLane<D, 1> at(p.tokens_per_page, 0, lane);
     uint8_t* const my_ring = smem + warp * (S * G::kSlotBytes);
     const uint8_t* const my_scales = scale_ring + warp * (S * G::kScaleBytes);
@@ -1222,21 +1212,21 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
     uint32_t slot = 0, phase = 0;
     bool ok = true;
 
-    scaled_share<G>(p, a, cells, row_blocks, reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(stat_m), share);
+    scaled_share<G>(p, a, cells, reinterpret_cast<uint32_t*>(smem), reinterpret_cast<uint32_t*>(stat_m), share);
     uint32_t group = share->first, first_item = 0;
     while (group <= share->last) {
         const ScaledRun run = share->run(group, a.templates);
-        const uint32_t run_items = run.templates * row_blocks;
+        const uint32_t run_items = run.templates;
         if (first_item >= run_items) {
             ++group;
             first_item = 0;
             continue;
         }
         const uint32_t seen = min(uint32_t(G::kItems), run_items - first_item);
-        for (uint32_t i = tid; i < seen; i += G::kThreads) items[i] = scaled_item<1>(p, a, run, first_item + i, G::kRows, row_blocks);
+        for (uint32_t i = tid; i < seen; i += G::kThreads) items[i] = scaled_item<1>(p, a, run, first_item + i);
         __syncthreads();
         if (warp == 0) {
-            const uint32_t kept = scaled_chains<true>(p, run, items, cum, seen, first_item + seen < run_items, row_blocks, lane);
+            const uint32_t kept = scaled_chains<true>(p, run, items, cum, seen, first_item + seen < run_items, lane);
             if (lane == 0) *pass_items = kept;
         }
         __syncthreads();
