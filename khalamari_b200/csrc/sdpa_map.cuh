@@ -338,12 +338,13 @@ __device__ __forceinline__ void merge_state_combine(MergeState& state, const Mer
     state.max = new_max;
 }
 
-// Normalised output of a merged row; writes the merged statistics when asked.
+// Normalised output of a merged row; writes the merged statistics when asked. A NaN sum keeps its finite maximum: a
+// second merge skips records without one.
 __device__ __forceinline__ float4 merge_state_finish(const MergeState& state, float* out_sum, float* out_max) {
     const float inv = state.sum > 0.0f ? 1.0f / state.sum : 0.0f;
     if (out_sum != nullptr) {
         *out_sum = state.sum;
-        *out_max = state.sum > 0.0f ? state.max : -INFINITY;
+        *out_max = state.sum == 0.0f ? -INFINITY : state.max;
     }
     return make_float4(state.acc.x * inv, state.acc.y * inv, state.acc.z * inv, state.acc.w * inv);
 }
