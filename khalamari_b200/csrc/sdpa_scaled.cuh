@@ -491,7 +491,9 @@ struct ScaledLane {
 // Q fragments of n-tile n for one lane: row n * 8 + g, elements 128 (c / 2) + 32 t + 16 (c % 2) + (0 .. 15)
 // as f16 pairs, `put(step, pair)`.
 // bf16 rows are scaled by a power of two so that their largest element lies in [2^8, 2^9): exact in f16 down to 2^-22 of
-// that element, and no bf16 value overflows. Returns the factor from the row's dot products to log2-domain scores.
+// that element, and no bf16 value overflows. Returns the factor from the row's dot products to log2-domain scores; NaN for a
+// row that is not finite, whose softmax is NaN wherever it sees a token (left to the scores, a row of -inf would look like
+// one that sees nothing).
 template <typename T, int D, typename Put>
 __device__ __forceinline__ float scaled_load_q(const MapParams& p, const ScaledRows& rows, uint32_t n, uint32_t lane, Put put) {
     constexpr int KC = D / 64;
@@ -510,21 +512,25 @@ __device__ __forceinline__ float scaled_load_q(const MapParams& p, const ScaledR
         for (int c = 0; c < KC; ++c) raw[c][0] = raw[c][1] = make_uint4(0, 0, 0, 0);
     }
     float factor = p.scale_log2e, up = 1.0f;
-    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        uint32_t most = 0;
+    uint32_t most = 0;  // the row's largest magnitude bits (ordered as integers)
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
+    for (int c = 0; c < KC; ++c) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                most = __vmaxu2(most, __vmaxu2(__vmaxu2(raw[c][h].x & 0x7fff7fffu, raw[c][h].y & 0x7fff7fffu),
-                                               __vmaxu2(raw[c][h].z & 0x7fff7fffu, raw[c][h].w & 0x7fff7fffu)));
-            }
+        for (int h = 0; h < 2; ++h) {
+            most = __vmaxu2(most, __vmaxu2(__vmaxu2(raw[c][h].x & 0x7fff7fffu, raw[c][h].y & 0x7fff7fffu),
+                                           __vmaxu2(raw[c][h].z & 0x7fff7fffu, raw[c][h].w & 0x7fff7fffu)));
         }
-        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
-        most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
-        const int exponent = int(max(most & 0xffffu, most >> 16) >> 7);  // of the largest element, biased
-        if (exponent >= 9 && exponent < 255) {  // (tinier rows, and rows with a NaN or an infinity, go as they are)
-            up = __uint_as_float(uint32_t(262 - exponent) << 23);        // 2^(8 - k), k = exponent - 127
+    }
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 1));
+    most = __vmaxu2(most, __shfl_xor_sync(0xffffffffu, most, 2));
+    most = max(most & 0xffffu, most >> 16);
+    constexpr uint32_t kInfinity = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    if (most >= kInfinity) {
+        factor = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all scores of the row are NaN or infinite
+    } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        const int exponent = int(most >> 7);  // of the largest element, biased
+        if (exponent >= 9) {                  // (tinier rows go as they are)
+            up = __uint_as_float(uint32_t(262 - exponent) << 23);  // 2^(8 - k), k = exponent - 127
             factor = p.scale_log2e * __uint_as_float(uint32_t(exponent - 8) << 23);
         }
     }
@@ -774,8 +780,8 @@ __device__ __forceinline__ void scaled_publish_stats(const MapParams& p, const S
                                                      float m, float sum) {
     const uint64_t index = (uint64_t(chain->slot) * p.num_q_heads + rows.head(row)) * p.max_q_tokens + rows.token(row);
     p.partial_sum[index] = sum;
-    // natural-log domain; a NaN sum needs a finite maximum to reach the merged output
-    p.partial_max[index] = m > kScaledNothing ? m * 0.6931471805599453f : (sum == sum ? -INFINITY : 0.0f);
+    // natural-log domain; a NaN sum needs a finite maximum to reach the merged output, whatever its own is
+    p.partial_max[index] = sum != sum ? 0.0f : m > kScaledNothing ? m * 0.6931471805599453f : -INFINITY;
     for (uint32_t i = 1; i <= chain->empties; ++i) {
         const uint64_t other = index + uint64_t(i) * p.num_q_heads * p.max_q_tokens;
         p.partial_sum[other] = 0.0f;

@@ -704,6 +704,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             }
             if (!ok) break;
             // ---- epilogue
+            // (a token that is seen adds 1 at the maximum, unless every score is -inf: that softmax is NaN)
+            if (l == 0.0f && hi > lo) l = __uint_as_float(0x7fc00000u);
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;  // (a NaN sum stays NaN)
             const uint64_t index = (uint64_t(tmpl) * p.num_q_heads + head) * p.max_q_tokens + row_tok;
             if (steps > 0) {
@@ -744,8 +746,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             }
             if (valid && p.direct == 0) {
                 p.partial_sum[index] = l;
-                // natural-log domain; a NaN sum needs a finite maximum to reach the merged output
-                p.partial_max[index] = m > -INFINITY ? m * (p.scale_log2e * 0.6931471805599453f) : (l == l ? -INFINITY : 0.0f);
+                // natural-log domain; a NaN sum needs a finite maximum to reach the merged output, whatever its own is
+                p.partial_max[index] = l != l ? 0.0f : m > -INFINITY ? m * (p.scale_log2e * 0.6931471805599453f) : -INFINITY;
             }
             if (steps > 0) {
                 tmem_fence_before();
