@@ -3,7 +3,8 @@
 //   code of (plane, head, row, d):  page + ((plane * Hkv + head) * P + row) * D + d          plane 0 = K, 1 = V
 //   scale byte of the same row:     page + 2 * Hkv * P * D + (head * 2 + plane) * P + row
 // A row stands for code * 2^(b - 127). Powers of two, so that scaling a value into the codes' range, and a code back,
-// rounds nothing: the only rounding is the one to the code, and int8 or E4M3 codes times 2^e are exact in bf16. b = 0:
+// rounds nothing: the only rounding is the one to the code, and int8 or E4M3 codes times 2^e are exact in bf16 as far as
+// its range goes (a row of its largest value stands for 2^128, one of f16's for 2^16). b = 0:
 // a row of zeros. b = 255: a row with a NaN or an infinity; its codes are zeros, and 0 * inf = NaN on the way back.
 #pragma once
 
@@ -75,14 +76,18 @@ __device__ __forceinline__ void codes4_to_half(uint32_t word, uint32_t& lo, uint
 }
 
 // 2^(b - 127) as packed pairs of T, in two factors: f16 scales may lie below its smallest normal number, and the product
-// of a code with the first factor is exact. Where V's byte marks a row that is not finite its codes count as zeros (the
-// row's K is NaN, which is what reaches the queries that see it).
+// of a code with the first factor is exact. As an operand of P V (`v`) a bf16 row is taken 2^-kValueShift times its size,
+// for sums that stay inside f32 (rows below 2^-116 lose bits to that), and a row that is not finite counts as zeros (its
+// K is NaN, which is what reaches the queries that see it).
+constexpr uint32_t kValueShift = 10;
 template <typename T>
 __device__ __forceinline__ void scaled_factors(uint32_t b, bool v, uint32_t& first, uint32_t& second);
 template <>
 __device__ __forceinline__ void scaled_factors<__nv_bfloat16>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
     if (v && b == 255) b = 0;
-    first = (b << 7) * 0x00010001u;
+    // (below 2^-126 a subnormal power)
+    const uint32_t power = !v ? b << 7 : b > kValueShift ? (b - kValueShift) << 7 : 0x80u >> (kValueShift + 1 - b);
+    first = power * 0x00010001u;
     second = 0;
 }
 template <>
@@ -160,6 +165,14 @@ __device__ __forceinline__ uint32_t saturate2<__nv_bfloat16>(uint32_t v) {
     const __nv_bfloat162 most = __halves2bfloat162(__ushort_as_bfloat16(0x7f7f), __ushort_as_bfloat16(0x7f7f)), least = __hneg2(most);
     const __nv_bfloat162 cut = __hmin2_nan(__hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&v), least), most);
     return *reinterpret_cast<const uint32_t*>(&cut);
+}
+// The same in f32, at the largest value of T.
+template <typename T>
+__device__ __forceinline__ float saturate(float x) {
+    const float most = std::is_same<T, __half>::value ? 65504.0f : __uint_as_float(0x7f7f0000u);
+    asm("min.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(most));
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-most));
+    return x;
 }
 // Scale bytes from which a code can leave T's range (codes are below 2^9).
 template <typename T>

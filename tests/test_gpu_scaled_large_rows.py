@@ -1,0 +1,65 @@
+"""Scaled 8-bit pages and cached rows at the top of their type's range (``-m gpu``): a row of the type's largest value stands
+for one step more (2^128 from bf16, 2^16 from f16), which must not turn into infinities or NaN on the way."""
+import numpy as np
+import pytest
+
+from helpers import round_to
+from scaled_helpers import CODES, ScaledRun, assert_close, make_scaled_case, planes, quantise, reference, values_of
+
+pytestmark = pytest.mark.gpu
+
+MOST = {"bf16": float(np.uint32(0x7F7F0000).view(np.float32)), "f16": 65504.0}
+
+
+@pytest.fixture(scope="module")
+def device():
+    from khalamari_b200.device import Device
+    return Device(0)
+
+
+def _put(case, request, tokens, k=None, v=None):
+    """Replaces cached rows [len(tokens), Hkv, D] of one request: quantised here, as the page write does."""
+    codes, scales = planes(case.pool, case.hkv, case.page, case.d)
+    tokens = np.asarray(tokens)
+    at, row = case.table[case.slots[request], case.layer, tokens // case.page], tokens % case.page
+    for plane, (held, x) in enumerate(((case.k, k), (case.v, v))):
+        if x is None:
+            continue
+        _, x = round_to(case.dtype_name, np.broadcast_to(x, (len(tokens), case.hkv, case.d)).astype(np.float32))
+        c, b = quantise(x, case.code)
+        codes[at, plane, :, row] = c
+        scales[at, :, plane, row] = b
+        held[request] = held[request].copy()
+        held[request][tokens] = values_of(c, b, case.code)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d,histories,q_lens", [
+    (16, 2, 128, [300], [64]), (16, 2, 256, [300], [64]), (24, 4, 128, [40], [4]), (24, 4, 256, [40], [4]), (8, 8, 128, [0], [24]),
+])
+def test_a_largest_row_reaches_only_the_queries_that_see_it(device, code, io, hq, hkv, d, histories, q_lens):
+    """The new chunk's middle token holds V rows of the largest value: earlier queries share its step and must not see it."""
+    case = make_scaled_case(d + hq, code, io, hq, hkv, d, histories, q_lens)
+    middle = q_lens[0] // 2 + q_lens[0] // 12
+    _put(case, 0, [histories[0] + middle], v=MOST[io])
+    run = ScaledRun(device, case, max_tokens=256)
+    run.plan()
+    run.record()
+    out = run.read()
+    expected, bound = reference(case, wide=run.wide())
+    assert_close(out[:middle], expected[:middle], bound[:middle], "queries before the token")
+    assert not np.isnan(out).any()
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("io", ["bf16", "f16"])
+@pytest.mark.parametrize("hq,hkv,d,q_len", [(16, 2, 128, 64), (16, 2, 256, 64)])
+def test_an_average_of_largest_rows_is_the_largest_value(device, code, io, hq, hkv, d, q_len):
+    """All V rows alike: the output is that row, as it was before it was quantised."""
+    case = make_scaled_case(3, code, io, hq, hkv, d, [0], [q_len])
+    signs = np.where(np.arange(d) % 3 == 0, -1.0, 1.0)
+    _put(case, 0, np.arange(q_len), v=MOST[io] * signs)
+    out = ScaledRun(device, case, max_tokens=256).run()
+    # probabilities are rounded on their own (half a step each), the sum is not
+    assert np.all(np.abs(out / signs - MOST[io]) <= MOST[io] * 2.02 * (2.0 ** -8 if io == "bf16" else 2.0 ** -11))
