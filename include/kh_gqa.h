@@ -344,7 +344,9 @@ KH_API kh_status kh_metadata_update(const kh_metadata_arrays* arrays, const uint
  * metal/gqa_fp8.metal:1-25 does (16-token pages, head_dim 128 or 256). kv_dtype = dtype: the pages hold
  * Q/output-type elements. kv_dtype = KH_DTYPE_INT8_SCALED / KH_DTYPE_FP8_E4M3FN_SCALED: codes with a scale byte for
  * each (token, KV head) row (every (head_dim, tokens_per_page) profile; kv_pages and q 16-byte aligned; the
- * one-launch map + reduce form is not offered). */
+ * one-launch map + reduce form is not offered). Their partials carry an exp sum of 1 under the logarithm of the whole sum
+ * as maximum (0 and -inf where nothing is visible; NaN and 0 where a score is NaN), which any merge takes as it takes the
+ * others. Outputs saturate at the type's largest finite value, as the page read's do. */
 typedef struct kh_sliced_kv_config {
     uint32_t num_q_heads;
     uint32_t num_kv_heads;

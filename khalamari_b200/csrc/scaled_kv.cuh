@@ -174,6 +174,13 @@ __device__ __forceinline__ float saturate(float x) {
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(x) : "f"(-most));
     return x;
 }
+// Statistics of a published partial: a sum of 1 under the logarithm of the whole sum (0 and -inf of a row that sees nothing),
+// so that it weighs at most 1 in the merge and outputs near the type's largest value leave room for their sum. A NaN sum
+// needs a finite maximum to reach the merged output, whatever its own is. `m` and the sum in the natural-log domain.
+__device__ __forceinline__ void publish_partial_stats(float* partial_sum, float* partial_max, uint64_t index, float m, float sum) {
+    partial_sum[index] = sum != sum ? sum : sum == 0.0f ? 0.0f : 1.0f;
+    partial_max[index] = sum != sum ? 0.0f : sum == 0.0f ? -INFINITY : m + logf(sum);
+}
 // Scale bytes from which a code can leave T's range (codes are below 2^9).
 template <typename T>
 __device__ __forceinline__ constexpr uint32_t first_large_byte() { return std::is_same<T, __half>::value ? 134u : 246u; }

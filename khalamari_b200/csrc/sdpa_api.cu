@@ -16,6 +16,7 @@
 #include "cuda_objects.h"
 #include "host_sdpa.h"
 #include "map_instance.h"
+#include "scaled_kv.cuh"
 #include "sdpa_map.cuh"
 #include "sdpa_tc.cuh"
 #include "sdpa_tm.cuh"
@@ -50,6 +51,7 @@ struct ReduceParams {
     const uint32_t* active;    // replay: device words {tokens, Q-token tiles, templates}; the counts above bound them
     uint32_t active_range_word; // which of the words counts this launch's ranges (0: tokens, 1: Q-token tiles)
     uint32_t wide;             // long partial lists: the widest block, whose thread groups share a row's list
+    uint32_t saturate;         // scaled 8-bit pages: outputs stop at the type's largest value (scaled_kv.cuh)
 };
 
 template <typename T>
@@ -73,6 +75,12 @@ __device__ __forceinline__ void store4<__half>(__half* dst, float4 v) {
     *reinterpret_cast<uint2*>(dst) = packed;
 }
 
+template <typename T>
+__device__ __forceinline__ void store_reduced4(const ReduceParams& p, T* dst, float4 v) {
+    if (p.saturate != 0) v = make_float4(saturate<T>(v.x), saturate<T>(v.y), saturate<T>(v.z), saturate<T>(v.w));
+    store4<T>(dst, v);
+}
+
 constexpr uint32_t kReduceMaxThreads = 512;
 
 template <typename T>
@@ -89,6 +97,7 @@ __global__ void __launch_bounds__(kReduceMaxThreads) sdpa_reduce_kernel(const Re
         num_active_tokens = min(p.active[0], num_active_tokens);
     }
     if (range >= num_active_ranges) return;
+    const float unit = p.saturate != 0 ? 1.0f / 1024.0f : 1.0f;  // partials of scaled pages weigh at most 1 each
     if (p.heads_per_block > 1) {
         // decode shape: one token per range, few partials per row. A thread owns four output columns of one
         // head; no shared memory, no second wave of blocks.
@@ -107,9 +116,9 @@ __global__ void __launch_bounds__(kReduceMaxThreads) sdpa_reduce_kernel(const Re
         const uint64_t first_index = uint64_t(first) * p.num_q_heads + head;
         float merged_sum, merged_max;
         const float4 acc = merge_partials_vec(p.partial_sum, p.partial_max, p.partial_out, first_index, stride, out_stride,
-                                              last - first, D, d, &merged_sum, &merged_max);
+                                              last - first, D, d, &merged_sum, &merged_max, unit);
         const uint64_t out_row = uint64_t(tok) * p.num_q_heads + head;
-        store4<T>(reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
+        store_reduced4<T>(p, reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
         if (p.out_sum != nullptr && d == 0) {
             p.out_sum[out_row] = merged_sum;
             p.out_max[out_row] = merged_max;
@@ -141,9 +150,9 @@ __global__ void __launch_bounds__(kReduceMaxThreads) sdpa_reduce_kernel(const Re
             const uint64_t first_index = (uint64_t(first) * p.num_q_heads + head) * p.max_q_tokens + tok;
             float merged_sum, merged_max;
             const float4 acc = merge_partials_vec(p.partial_sum, p.partial_max, p.partial_out, first_index, stride,
-                                                  out_stride, last - first, D, d, &merged_sum, &merged_max);
+                                                  out_stride, last - first, D, d, &merged_sum, &merged_max, unit);
             const uint64_t out_row = uint64_t(tok_begin + tok) * p.num_q_heads + head;
-            store4<T>(reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
+            store_reduced4<T>(p, reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
             if (p.out_sum != nullptr && d == 0) {
                 p.out_sum[out_row] = merged_sum;
                 p.out_max[out_row] = merged_max;
@@ -164,7 +173,7 @@ __global__ void __launch_bounds__(kReduceMaxThreads) sdpa_reduce_kernel(const Re
         const uint64_t first_index = (uint64_t(first) * p.num_q_heads + head) * p.max_q_tokens + tok;
         merge_partials_accumulate(state, p.partial_sum + uint64_t(begin) * stride, p.partial_max + uint64_t(begin) * stride,
                                   p.partial_out + uint64_t(begin) * out_stride, first_index, stride, out_stride, mine,
-                                  D, d);
+                                  D, d, unit);
     }
     shared_acc[threadIdx.x] = state.acc;
     shared_stat[threadIdx.x] = make_float2(state.sum, state.max);
@@ -178,7 +187,7 @@ __global__ void __launch_bounds__(kReduceMaxThreads) sdpa_reduce_kernel(const Re
     float merged_sum, merged_max;
     const float4 acc = merge_state_finish(state, &merged_sum, &merged_max);
     const uint64_t out_row = uint64_t(tok_begin + tok) * p.num_q_heads + head;
-    store4<T>(reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
+    store_reduced4<T>(p, reinterpret_cast<T*>(p.out) + out_row * D + d, acc);
     if (p.out_sum != nullptr && d == 0) {
         p.out_sum[out_row] = merged_sum;
         p.out_max[out_row] = merged_max;
@@ -1168,6 +1177,7 @@ kh_status kh_sliced_kv_reduce(kh_sliced_kv* compute, kh_stream* stream, const kh
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 0;
+        p.saturate = is_scaled(compute->config.kv_dtype) ? 1 : 0;
         p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens, p.head_dim);
         launch_reduce(compute->config.dtype, p, num_active_tokens, stream->stream);
         return KH_OK;
@@ -1379,6 +1389,7 @@ kh_status kh_sliced_q_reduce(kh_sliced_q* compute, kh_stream* stream, const kh_s
         p.num_partials = s.num_total_sdpa_map_task_templates;
         p.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         p.active_range_word = 1;
+        p.saturate = is_scaled(compute->config.kv_dtype) ? 1 : 0;
         p.wide = wide_reduce(compute->config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_q_token_tiles,
                              p.max_q_tokens * p.head_dim);
         launch_reduce(compute->config.dtype, p, num_active_q_token_tiles, stream->stream);
@@ -1579,6 +1590,7 @@ kh_status kh_sliced_kv_attend_static(kh_sliced_kv* compute, kh_stream* stream,
         r.num_partials = num_active_kv_splits;  // the sections of the shared array are sized for exactly these
         r.active = static_cast<const uint32_t*>(stream->active_counts.ptr);
         r.active_range_word = 0;
+        r.saturate = is_scaled(config.kv_dtype) ? 1 : 0;
         r.wide = wide_reduce(config.kv_dtype, s.num_total_sdpa_map_task_templates, s.num_total_tokens, r.head_dim);
         launch_reduce(config.dtype, r, num_active_tokens, stream->stream);
         return KH_OK;

@@ -271,12 +271,13 @@ __device__ __forceinline__ MergeState merge_state_empty() {
     return MergeState{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY};
 }
 
-// Folds `count` partials of one row into `state`.
+// Folds `count` partials of one row into `state`. All weights are taken `unit` times their size, which the division by their
+// sum takes back: sums of outputs near the top of f32's range need it (powers of two only).
 __device__ __forceinline__ void merge_partials_accumulate(MergeState& state, const float* partial_sum,
                                                           const float* partial_max, const float* partial_out,
                                                           uint64_t first_index, uint64_t index_stride,
                                                           uint64_t out_stride, uint32_t count, uint32_t head_dim,
-                                                          uint32_t d) {
+                                                          uint32_t d, float unit = 1.0f) {
     float run_max = state.max, run_sum = state.sum;
     float4 acc = state.acc;
     for (uint32_t base = 0; base < count; base += 8) {
@@ -299,7 +300,7 @@ __device__ __forceinline__ void merge_partials_accumulate(MergeState& state, con
         float4 v[8];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            weight[j] = (sm[j] != 0.0f && isfinite(mx[j])) ? expf(mx[j] - new_max) * sm[j] : 0.0f;
+            weight[j] = (sm[j] != 0.0f && isfinite(mx[j])) ? expf(mx[j] - new_max) * (sm[j] * unit) : 0.0f;
             const uint64_t out_index = first_index * head_dim + uint64_t(base + j) * out_stride + d;
             v[j] = weight[j] != 0.0f ? __ldcg(reinterpret_cast<const float4*>(partial_out + out_index))
                                      : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -352,10 +353,11 @@ __device__ __forceinline__ float4 merge_state_finish(const MergeState& state, fl
 __device__ __forceinline__ float4 merge_partials_vec(const float* partial_sum, const float* partial_max,
                                                      const float* partial_out, uint64_t first_index,
                                                      uint64_t index_stride, uint64_t out_stride, uint32_t count,
-                                                     uint32_t head_dim, uint32_t d, float* out_sum, float* out_max) {
+                                                     uint32_t head_dim, uint32_t d, float* out_sum, float* out_max,
+                                                     float unit = 1.0f) {
     MergeState state = merge_state_empty();
     merge_partials_accumulate(state, partial_sum, partial_max, partial_out, first_index, index_stride, out_stride,
-                              count, head_dim, d);
+                              count, head_dim, d, unit);
     return merge_state_finish(state, out_sum, out_max);
 }
 

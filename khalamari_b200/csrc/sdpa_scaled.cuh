@@ -779,9 +779,7 @@ __device__ __forceinline__ void scaled_tiles(const MapParams& p, ScaledState<D, 
 __device__ __forceinline__ void scaled_publish_stats(const MapParams& p, const ScaledRows& rows, const ScaledItem* chain, uint32_t row,
                                                      float m, float sum) {
     const uint64_t index = (uint64_t(chain->slot) * p.num_q_heads + rows.head(row)) * p.max_q_tokens + rows.token(row);
-    p.partial_sum[index] = sum;
-    // natural-log domain; a NaN sum needs a finite maximum to reach the merged output, whatever its own is
-    p.partial_max[index] = sum != sum ? 0.0f : m > kScaledNothing ? m * 0.6931471805599453f : -INFINITY;
+    publish_partial_stats(p.partial_sum, p.partial_max, index, m * 0.6931471805599453f, sum);
     for (uint32_t i = 1; i <= chain->empties; ++i) {
         const uint64_t other = index + uint64_t(i) * p.num_q_heads * p.max_q_tokens;
         p.partial_sum[other] = 0.0f;
@@ -789,12 +787,22 @@ __device__ __forceinline__ void scaled_publish_stats(const MapParams& p, const S
     }
 }
 
-// Where four consecutive output elements of a row go: the final output, or the chain's partial slot.
-template <typename T, int D>
+// The factor 2^(r - m) / sum from accumulators to outputs is taken in two, 2^up first: m may lag by 2^8 behind a largest score
+// and V's exponents reach 2^122, while f32 ends at 2^128. An output may be 2^128 all the same (what codes of a bf16 row's
+// largest value stand for): as a partial it must stay finite, so such large ones are taken 2^-20 smaller.
+__device__ __forceinline__ float scaled_rise(float r, float m) { return r - m > 96.0f ? 32.0f : 0.0f; }
+__device__ __forceinline__ float scaled_last_factor(float r, float m, float up, float sum) {
+    const float f = sum == 0.0f ? 0.0f : fast_exp2(r - m - up) / sum;  // (a NaN sum stays NaN)
+    return up > 0.0f ? f * (1.0f - 0x1p-20f) : f;
+}
+
+// Four consecutive output elements of a row into the final output, or into the chain's partial slot.
+template <typename T, int D, bool DIRECT>
 __device__ __forceinline__ void scaled_publish4(const MapParams& p, const ScaledRows& rows, const ScaledItem* chain, uint32_t row, uint32_t d,
                                                 float4 v) {
-    if (p.direct != 0) {
-        store_out4<T>(static_cast<T*>(p.out) + ((uint64_t(rows.tok_begin) + rows.token(row)) * p.num_q_heads + rows.head(row)) * D + d, v);
+    if constexpr (DIRECT) {
+        T* const dst = static_cast<T*>(p.out) + ((uint64_t(rows.tok_begin) + rows.token(row)) * p.num_q_heads + rows.head(row)) * D + d;
+        *reinterpret_cast<uint2*>(dst) = make_uint2(saturate2<T>(pack2<T>(v.x, v.y)), saturate2<T>(pack2<T>(v.z, v.w)));
     } else {
         const uint64_t index = (uint64_t(chain->slot) * p.num_q_heads + rows.head(row)) * p.max_q_tokens + rows.token(row);
         *reinterpret_cast<float4*>(p.partial_out + index * D + d) = v;
@@ -982,7 +990,7 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
             for (uint32_t x = lane; x < uint32_t(G::kRows * (D / 4)); x += 32) {
                 const uint32_t row = x / (D / 4);
                 if (!rows.valid(row)) continue;
-                if (p.direct != 0) scaled_publish4<T, D>(p, rows, &it, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
+                if (p.direct != 0) scaled_publish4<T, D, true>(p, rows, &it, row, x % (D / 4) * 4, make_float4(0.0f, 0.0f, 0.0f, 0.0f));
                 else if (x % (D / 4) == 0) scaled_publish_stats(p, rows, &it, row, kScaledNothing, 0.0f);
             }
         }
@@ -1002,15 +1010,20 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
                     const uint32_t row = n * 8 + 2 * t + c;
                     if (!rows.valid(row)) continue;
                     const float sum = st.l[n][c];
-                    // (a NaN sum stays NaN)
-                    const float f = sum == 0.0f ? 0.0f : fast_exp2(st.r[n][c] - st.m[n][c]) / sum;
+                    const float up = scaled_rise(st.r[n][c], st.m[n][c]), raise = fast_exp2(up);
+                    const float f = scaled_last_factor(st.r[n][c], st.m[n][c], up, sum);
+                    auto part = [&](int j) {
+                        return make_float4(st.acc[n][j][c] * raise * f, st.acc[n][j][2 + c] * raise * f, st.acc[n][j + 1][c] * raise * f,
+                                           st.acc[n][j + 1][2 + c] * raise * f);
+                    };
+                    if (p.direct != 0) {
 #pragma unroll
-                    for (int j = 0; j < KS; j += 2) {
-                        scaled_publish4<T, D>(p, rows, first, row, (j / 8) * 128 + g * 16 + (j % 8) * 2,
-                                              make_float4(st.acc[n][j][c] * f, st.acc[n][j][2 + c] * f, st.acc[n][j + 1][c] * f,
-                                                          st.acc[n][j + 1][2 + c] * f));
+                        for (int j = 0; j < KS; j += 2) scaled_publish4<T, D, true>(p, rows, first, row, (j / 8) * 128 + g * 16 + (j % 8) * 2, part(j));
+                        continue;
                     }
-                    if (g == 0 && p.direct == 0) scaled_publish_stats(p, rows, first, row, st.m[n][c], sum);
+#pragma unroll
+                    for (int j = 0; j < KS; j += 2) scaled_publish4<T, D, false>(p, rows, first, row, (j / 8) * 128 + g * 16 + (j % 8) * 2, part(j));
+                    if (g == 0) scaled_publish_stats(p, rows, first, row, st.m[n][c], sum);
                 }
             }
         };
@@ -1180,7 +1193,7 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
     float* const stat_l = stat_r + W * G::kRows;
     float* const row_factor = stat_l + W * G::kRows;  // [rows] from dot products to scores
     float* const row_out = row_factor + G::kRows;     // [rows] final factor of the merged accumulators
-    float* const row_ref = row_out + G::kRows;        // [rows] merged value reference
+    float* const row_ref = row_out + G::kRows;        // [rows] reference of the merged accumulators
     uint8_t* const scale_ring = reinterpret_cast<uint8_t*>(stat_m) + G::kStatBytes;
     uint64_t* const bars = reinterpret_cast<uint64_t*>(scale_ring + W * S * G::kScaleBytes);
     uint2* const infos = reinterpret_cast<uint2*>(bars + W * S * 2);
@@ -1307,8 +1320,9 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
                 top_r = fmaxf(top_r, stat_r[w * G::kRows + row]);
             }
             for (int w = 0; w < W; ++w) sum += stat_l[w * G::kRows + row] * fast_exp2(stat_m[w * G::kRows + row] - top_m);
-            row_ref[row] = top_r;
-            row_out[row] = sum == 0.0f ? 0.0f : fast_exp2(top_r - top_m) / sum;  // (a NaN sum stays NaN)
+            const float up = scaled_rise(top_r, top_m);
+            row_ref[row] = top_r - up;
+            row_out[row] = scaled_last_factor(top_r, top_m, up, sum);
             if (p.direct == 0 && rows.valid(row)) scaled_publish_stats(p, rows, items, row, top_m, sum);
         }
         __syncthreads();
@@ -1338,7 +1352,9 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
                 }
                 if (rows.valid(n * 8 + row)) {
                     const float f = row_out[n * 8 + row];
-                    scaled_publish4<T, D>(p, rows, items, n * 8 + row, d, make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f));
+                    const float4 v = make_float4(sum.x * f, sum.y * f, sum.z * f, sum.w * f);
+                    if (p.direct != 0) scaled_publish4<T, D, true>(p, rows, items, n * 8 + row, d, v);
+                    else scaled_publish4<T, D, false>(p, rows, items, n * 8 + row, d, v);
                 }
             }
             __syncthreads();

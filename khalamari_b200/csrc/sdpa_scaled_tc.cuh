@@ -753,9 +753,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 }
             }
             if (valid && p.direct == 0) {
-                p.partial_sum[index] = l;
-                // natural-log domain; a NaN sum needs a finite maximum to reach the merged output, whatever its own is
-                p.partial_max[index] = l != l ? 0.0f : m > -INFINITY ? m * (p.scale_log2e * 0.6931471805599453f) : -INFINITY;
+                publish_partial_stats(p.partial_sum, p.partial_max, index, m * (p.scale_log2e * 0.6931471805599453f), l);
             }
             if (steps > 0) {
                 tmem_fence_before();
