@@ -92,6 +92,11 @@ inline uint64_t kv_row_bytes(kh_dtype kv_dtype, uint32_t head_dim) {
     return uint64_t(head_dim) * dtype_size(kv_dtype) + (is_scaled(kv_dtype) ? 1 : 0);
 }
 
+// Q rows up to which a Map task over scaled pages runs on the kernels that merge neighbouring slices of the same rows before
+// they publish them (sdpa_scaled.cuh: a row's accumulators are registers, head_dim of them); wider tasks go to
+// sdpa_scaled_tc.cuh, which publishes every slice. The dispatch and the selector's slices both go by it.
+inline uint32_t scaled_merging_rows(uint32_t head_dim) { return head_dim == 128 ? 32 : 24; }
+
 // What the kernels of scaled pages are built for (16-byte code rows, 8-byte groups of scale bytes).
 inline void require_scaled_profile(uint32_t head_dim, uint32_t tokens_per_page) {
     KH_REQUIRE(head_dim == 128 || head_dim == 256, "scaled 8-bit pages: head_dim 128 and 256 only (got %u)", head_dim);

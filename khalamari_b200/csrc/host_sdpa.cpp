@@ -468,11 +468,13 @@ Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* request
             tiles_total += tiles;
             work += (unsigned __int128)tiles * (requests[r].num_history_tokens + requests[r].num_q_tokens);
         }
-        // The chained kernels' wide tiles (more than 32 rows) are whole from fewer tasks on: at head_dim 128 two
+        // Tiles too wide for the kernels that merge slices are whole from fewer tasks on: at head_dim 128 two
         // neighbouring tiles share every K/V step at the price of one, which cutting the KV range would give up
         // (2,048 tokens behind 3,900, 64 / 8 heads: 806 us cut, 437 us whole), and at 256 the partials of cut tiles cost
-        // more than a last round that is half empty (2 x 2,048 tokens behind 4,000, 32 / 4 heads: 1,320 us cut, 894 us whole).
-        const bool wide = chained && variant.max_q_tokens * variant.max_q_heads > 32;
+        // more than a last round that is half empty (2 x 2,048 tokens behind 4,000, 32 / 4 heads: 1,320 us cut, 894 us whole); 4 / 4
+        // heads, tiles of 32 rows: 1,150 and 580 us).
+        const bool merges = chained && variant.max_q_tokens * variant.max_q_heads <= scaled_merging_rows(c.head_dim);
+        const bool wide = chained && !merges;
         const uint32_t whole = !wide ? kTasksPerSm : c.head_dim == 128 ? 1 : 2;
         if (sliced_q && tiles_total * head_groups >= uint64_t(sm_count) * whole) {
             // enough (Q tile, head group) tasks to fill every SM several times over without cutting the KV range:
@@ -481,8 +483,9 @@ Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* request
         } else {
             // A map kernel that merges neighbouring slices of the same rows before it publishes them pays nothing for
             // short slices and balances better with them (64 decode sequences over 8-bit pages: 512-token slices
-            // instead of 2,048 leave no SM more than 3 % behind instead of 13 %).
-            const uint32_t finer = chained && variant.max_q_tokens * variant.max_q_heads <= 32 ? 4 : 1;
+            // instead of 2,048 leave no SM more than 3 % behind instead of 13 %). The others pay with a partial for
+            // every slice (32 x 4 tokens behind 16,000, 16 / 2 heads of 256, tiles of 32 rows: 550 us finer, 407 us not).
+            const uint32_t finer = merges ? 4 : 1;
             slice = decode_slice(end, work * head_groups, min_slice, 2048,
                                  (unsigned __int128)sm_count * (sliced_q ? kTasksPerSm : kDecodeTasksPerSm) * finer);
             if (finer > 1) {

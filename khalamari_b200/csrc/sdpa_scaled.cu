@@ -29,22 +29,21 @@ static MapInstance make_tc_instance() {
 }
 
 // Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM; wider tasks go to tcgen05, whose
-// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 496 us here, 856 us there). `paired`: the KV heads can be taken two at a time (64 decode sequences:
-// 145 us, one at a time 150 us).
+// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 496 us here, 856 us there). `paired`: the
+// KV heads can be taken two at a time (64 decode sequences: 145 us, one at a time 150 us).
 template <typename T, int CODE, int D>
 static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {
+    if (rows > scaled_merging_rows(D)) return make_tc_instance<T, CODE, D>();
     if constexpr (D == 128) {
         if (rows <= 8 && paired) return make_stream_instance<T, CODE, 128, 1, 12, 2, 1>();
         if (rows <= 8) return make_stream_instance<T, CODE, 128, 1, 12, 1, 1>();
         if (rows <= 16) return make_stream_instance<T, CODE, 128, 2, 8, 1, 1>();
         if (rows <= 24) return make_chain_instance<T, CODE, 128, 3, 8>();
-        if (rows <= 32) return make_chain_instance<T, CODE, 128, 4, 8>();
-        return make_tc_instance<T, CODE, 128>();
+        return make_chain_instance<T, CODE, 128, 4, 8>();
     } else {
         if (rows <= 8) return make_stream_instance<T, CODE, 256, 1, 8, 1, 1>();
         if (rows <= 16) return make_chain_instance<T, CODE, 256, 2, 8>();
-        if (rows <= 24) return make_chain_instance<T, CODE, 256, 3, 8>();
-        return make_tc_instance<T, CODE, 256>();
+        return make_chain_instance<T, CODE, 256, 3, 8>();
     }
 }
 
