@@ -471,7 +471,7 @@ Route lookup_route_b200(const kh_sdpa_config& c, const kh_request_shape* request
         // Tiles too wide for the kernels that merge slices are whole from fewer tasks on: at head_dim 128 two
         // neighbouring tiles share every K/V step at the price of one, which cutting the KV range would give up
         // (2,048 tokens behind 3,900, 64 / 8 heads: 806 us cut, 437 us whole), and at 256 the partials of cut tiles cost
-        // more than a last round that is half empty (2 x 2,048 tokens behind 4,000, 32 / 4 heads: 1,320 us cut, 894 us whole); 4 / 4
+        // more than a last round that is half empty (2 x 2,048 tokens behind 4,000, 32 / 4 heads: 1,320 us cut, 894 us whole; 4 / 4
         // heads, tiles of 32 rows: 1,150 and 580 us).
         const bool merges = chained && variant.max_q_tokens * variant.max_q_heads <= scaled_merging_rows(c.head_dim);
         const bool wide = chained && !merges;

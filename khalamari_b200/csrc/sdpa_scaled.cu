@@ -9,10 +9,10 @@
 
 namespace kh {
 
-template <typename T, int CODE, int D, int NQ, int W, int HP, int NT>
+template <typename T, int CODE, int D, int NQ, int W, int HP>
 static MapInstance make_stream_instance() {
     using G = ScaledGeometry<D, NQ, W, HP, true>;
-    return MapInstance{sdpa_scaled_stream_kernel<T, CODE, D, NQ, W, HP, NT>, G::kThreads, G::kSmemBytes, G::kTileTokens, HP * 16,
+    return MapInstance{sdpa_scaled_stream_kernel<T, CODE, D, NQ, W, HP>, G::kThreads, G::kSmemBytes, G::kTileTokens, HP * 16,
                        G::kSlots};
 }
 
@@ -35,13 +35,13 @@ template <typename T, int CODE, int D>
 static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {
     if (rows > scaled_merging_rows(D)) return make_tc_instance<T, CODE, D>();
     if constexpr (D == 128) {
-        if (rows <= 8 && paired) return make_stream_instance<T, CODE, 128, 1, 12, 2, 1>();
-        if (rows <= 8) return make_stream_instance<T, CODE, 128, 1, 12, 1, 1>();
-        if (rows <= 16) return make_stream_instance<T, CODE, 128, 2, 8, 1, 1>();
+        if (rows <= 8 && paired) return make_stream_instance<T, CODE, 128, 1, 12, 2>();
+        if (rows <= 8) return make_stream_instance<T, CODE, 128, 1, 12, 1>();
+        if (rows <= 16) return make_stream_instance<T, CODE, 128, 2, 8, 1>();
         if (rows <= 24) return make_chain_instance<T, CODE, 128, 3, 8>();
         return make_chain_instance<T, CODE, 128, 4, 8>();
     } else {
-        if (rows <= 8) return make_stream_instance<T, CODE, 256, 1, 8, 1, 1>();
+        if (rows <= 8) return make_stream_instance<T, CODE, 256, 1, 8, 1>();
         if (rows <= 16) return make_chain_instance<T, CODE, 256, 2, 8>();
         return make_chain_instance<T, CODE, 256, 3, 8>();
     }

@@ -579,126 +579,107 @@ struct ScaledState {
     }
 };
 
-// NT tiles of 16 tokens into the state (two side by side hide each other's latencies). For tile i: `slot[i]` its codes,
-// `scales[i]` its scale bytes, `info[i]` its numbers (ScaledFetch). q(n, step): Q fragment.
-template <int CODE, int D, int NQ, int NT, int HP, typename Q>
-__device__ __forceinline__ void scaled_tiles(const MapParams& p, ScaledState<D, NQ>& st, uint8_t* const (&slot)[NT],
-                                             const uint8_t* const (&scales)[NT], const uint2 (&info)[NT], const ScaledItem* items,
-                                             uint32_t pair, const ScaledLane<D, HP>& at, uint32_t lane, Q q) {
+// A tile of 16 tokens into the state. `slot`: its codes, `scales`: its scale bytes, `info`: its numbers (ScaledFetch).
+// q(n, step): Q fragment.
+template <int CODE, int D, int NQ, int HP, typename Q>
+__device__ __forceinline__ void scaled_tile(const MapParams& p, ScaledState<D, NQ>& st, uint8_t* slot, const uint8_t* scales, uint2 info,
+                                            const ScaledItem* items, uint32_t pair, const ScaledLane<D, HP>& at, uint32_t lane, Q q) {
     constexpr int KC = D / 64, VG = D / 128;
-    constexpr int KA = NQ == 1 && NT == 1 ? 2 : 1;  // accumulators of a score tile: one chain of MMAs alone would wait on itself
-    constexpr float kMost = 256.0f;                 // a reference is raised when a weight would exceed this
+    constexpr int KA = NQ == 1 ? 2 : 1;  // accumulators of a score tile: one chain of MMAs alone would wait on itself
+    constexpr float kMost = 256.0f;      // a reference is raised when a weight would exceed this
     const uint32_t g = lane >> 2, t = lane & 3;
-    float k_scale[NT][2], v_log[NT][2];
+    float k_scale[2], v_log[2];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            k_scale[i][h] = scale_of_byte(scales[i][at.scale[h]]);
-            // b - 127 through the mantissa of 2^23 + b
-            v_log[i][h] = __uint_as_float(0x4b000000u | scales[i][at.scale[h] + at.v_scale]) - 8388735.0f;
-        }
+    for (int h = 0; h < 2; ++h) {
+        k_scale[h] = scale_of_byte(scales[at.scale[h]]);
+        // b - 127 through the mantissa of 2^23 + b
+        v_log[h] = __uint_as_float(0x4b000000u | scales[at.scale[h] + at.v_scale]) - 8388735.0f;
     }
 
     // ---- S^T = K Q^T
-    float s[NT][NQ][4], odd[KA == 2 ? 4 : 1];
+    float s[NQ][4], odd[KA == 2 ? 4 : 1];
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) s[i][n][0] = s[i][n][1] = s[i][n][2] = s[i][n][3] = 0.0f;
-    }
+    for (int n = 0; n < NQ; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
     if constexpr (KA == 2) odd[0] = odd[1] = odd[2] = odd[3] = 0.0f;
 #pragma unroll
     for (int c = 0; c < KC; ++c) {
-        uint32_t w0[NT][4], w1[NT][4];
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-            const uint32_t line = c / 2 * at.line, flip = c % 2 * 16;
-            const uint4 k0 = *reinterpret_cast<const uint4*>(slot[i] + line + (at.k[0] ^ flip));
-            const uint4 k1 = *reinterpret_cast<const uint4*>(slot[i] + line + (at.k[1] ^ flip));
-            w0[i][0] = k0.x, w0[i][1] = k0.y, w0[i][2] = k0.z, w0[i][3] = k0.w;
-            w1[i][0] = k1.x, w1[i][1] = k1.y, w1[i][2] = k1.z, w1[i][3] = k1.w;
-        }
+        uint32_t w0[4], w1[4];
+        const uint32_t line = c / 2 * at.line, flip = c % 2 * 16;
+        const uint4 k0 = *reinterpret_cast<const uint4*>(slot + line + (at.k[0] ^ flip));
+        const uint4 k1 = *reinterpret_cast<const uint4*>(slot + line + (at.k[1] ^ flip));
+        w0[0] = k0.x, w0[1] = k0.y, w0[2] = k0.z, w0[3] = k0.w;
+        w1[0] = k1.x, w1[1] = k1.y, w1[2] = k1.z, w1[3] = k1.w;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
+            uint32_t frag[4];
+            codes4_to_half<CODE>(w0[w], frag[0], frag[2]);
+            codes4_to_half<CODE>(w1[w], frag[1], frag[3]);
 #pragma unroll
-            for (int i = 0; i < NT; ++i) {
-                uint32_t frag[4];
-                codes4_to_half<CODE>(w0[i][w], frag[0], frag[2]);
-                codes4_to_half<CODE>(w1[i][w], frag[1], frag[3]);
-#pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    const uint2 b = q(n, c * 4 + w);
-                    if constexpr (KA == 2) {
-                        if (w & 1) mma_16816<__half>(odd, frag, b.x, b.y);
-                        else mma_16816<__half>(s[i][n], frag, b.x, b.y);
-                    } else {
-                        mma_16816<__half>(s[i][n], frag, b.x, b.y);
-                    }
+            for (int n = 0; n < NQ; ++n) {
+                const uint2 b = q(n, c * 4 + w);
+                if constexpr (KA == 2) {
+                    if (w & 1) mma_16816<__half>(odd, frag, b.x, b.y);
+                    else mma_16816<__half>(s[n], frag, b.x, b.y);
+                } else {
+                    mma_16816<__half>(s[n], frag, b.x, b.y);
                 }
             }
         }
     }
     if constexpr (KA == 2) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[0][0][e] += odd[e];
+        for (int e = 0; e < 4; ++e) s[0][e] += odd[e];
     }
     // ---- scores in the log2 domain: lane (g, t) holds tokens g, g + 8 (s[0..1], s[2..3]) of rows 2t, 2t + 1
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
+    for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] *= k_scale[e / 2] * st.factor[n][e % 2];
+    }
+    if ((info.x >> 31) == 0) {  // some row does not see all 16 tokens
+        const ScaledItem& item = items[info.x & 0xffu];
+        const uint32_t tok = info.y;
+        const ScaledRows rows(p, item, pair);
+        const uint32_t tmpl_begin = p.templates[uint64_t(item.tmpl) * 3 + 1], tmpl_end = p.templates[uint64_t(item.tmpl) * 3 + 2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[i][n][e] *= k_scale[i][e / 2] * st.factor[n][e % 2];
+            for (int c = 0; c < 2; ++c) {
+                const uint32_t row = n * 8 + 2 * t + c;
+                uint32_t lo = 0, hi = 0;
+                if (rows.valid(row)) scaled_visible(p, rows.tok_begin, rows.token(row), tmpl_begin, tmpl_end, lo, hi);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const uint32_t token = tok + 8 * h + g;
+                    if (token < lo || token >= hi) s[n][2 * h + c] = -INFINITY;
+                }
+            }
         }
-        if ((info[i].x >> 31) == 0) {  // some row does not see all 16 tokens
-            const ScaledItem& item = items[info[i].x & 0xffu];
-            const uint32_t tok = info[i].y;
-            const ScaledRows rows(p, item, pair);
-            const uint32_t tmpl_begin = p.templates[uint64_t(item.tmpl) * 3 + 1], tmpl_end = p.templates[uint64_t(item.tmpl) * 3 + 2];
+        if constexpr (CODE == kCodeE4M3) {
+            // rows outside the item may hold anything, the NaN code among it, and 0 * NaN is NaN
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
+            for (int r = 0; r < 4; ++r) {
+                const uint32_t token = tok + (r / 2) * 8 + 2 * t + r % 2;
+                if (token < item.kv_begin || token >= item.kv_end) {
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const uint32_t row = n * 8 + 2 * t + c;
-                    uint32_t lo = 0, hi = 0;
-                    if (rows.valid(row)) scaled_visible(p, rows.tok_begin, rows.token(row), tmpl_begin, tmpl_end, lo, hi);
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const uint32_t token = tok + 8 * h + g;
-                        if (token < lo || token >= hi) s[i][n][2 * h + c] = -INFINITY;
+                    for (int c = 0; c < VG; ++c) {
+                        *reinterpret_cast<uint4*>(slot + c * at.line + (at.v[r / 2] ^ (r % 2 * 16)) + r % 2 * 128) = make_uint4(0, 0, 0, 0);
                     }
                 }
             }
-            if constexpr (CODE == kCodeE4M3) {
-                // rows outside the item may hold anything, the NaN code among it, and 0 * NaN is NaN
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t token = tok + (r / 2) * 8 + 2 * t + r % 2;
-                    if (token < item.kv_begin || token >= item.kv_end) {
-#pragma unroll
-                        for (int c = 0; c < VG; ++c) {
-                            *reinterpret_cast<uint4*>(slot[i] + c * at.line + (at.v[r / 2] ^ (r % 2 * 16)) + r % 2 * 128) = make_uint4(0, 0, 0, 0);
-                        }
-                    }
-                }
-                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the slot's next copy lands after these
-            }
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // the slot's next copy lands after these
         }
     }
     // ---- probabilities (for the sum) and value weights, relative to the references
-    float pr[NT][NQ][4], w[NT][NQ][4], most = 0.0f;
+    float pr[NQ][4], w[NQ][4], most = 0.0f;
     auto weights = [&]() {
 #pragma unroll
-        for (int i = 0; i < NT; ++i) {
+        for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    pr[i][n][e] = fast_exp2(s[i][n][e] - st.m[n][e % 2]);
-                    w[i][n][e] = fast_exp2(s[i][n][e] + (v_log[i][e / 2] - st.r[n][e % 2]));
-                    most = fmaxf(most, fmaxf(pr[i][n][e], w[i][n][e]));
-                }
+            for (int e = 0; e < 4; ++e) {
+                pr[n][e] = fast_exp2(s[n][e] - st.m[n][e % 2]);
+                w[n][e] = fast_exp2(s[n][e] + (v_log[e / 2] - st.r[n][e % 2]));
+                most = fmaxf(most, fmaxf(pr[n][e], w[n][e]));
             }
         }
     };
@@ -708,12 +689,8 @@ __device__ __forceinline__ void scaled_tiles(const MapParams& p, ScaledState<D, 
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
             for (int c = 0; c < 2; ++c) {
-                float top_s = kScaledNothing, top_y = kScaledNothing;
-#pragma unroll
-                for (int i = 0; i < NT; ++i) {
-                    top_s = fmaxf(top_s, fmaxf(s[i][n][c], s[i][n][2 + c]));
-                    top_y = fmaxf(top_y, fmaxf(s[i][n][c] + v_log[i][0], s[i][n][2 + c] + v_log[i][1]));
-                }
+                float top_s = fmaxf(kScaledNothing, fmaxf(s[n][c], s[n][2 + c]));
+                float top_y = fmaxf(kScaledNothing, fmaxf(s[n][c] + v_log[0], s[n][2 + c] + v_log[1]));
 #pragma unroll
                 for (int d = 4; d <= 16; d <<= 1) {
                     top_s = fmaxf(top_s, __shfl_xor_sync(0xffffffffu, top_s, d));
@@ -736,40 +713,34 @@ __device__ __forceinline__ void scaled_tiles(const MapParams& p, ScaledState<D, 
         }
         weights();
     }
-    uint32_t weight[NT][NQ][2];  // B fragments: packed pairs of rows, transposed
+    uint32_t weight[NQ][2];  // B fragments: packed pairs of rows, transposed
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-#pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-            st.l[n][0] += pr[i][n][0] + pr[i][n][2];
-            st.l[n][1] += pr[i][n][1] + pr[i][n][3];
-            weight[i][n][0] = movmatrix_trans(pack2<__half>(w[i][n][0], w[i][n][1]));
-            weight[i][n][1] = movmatrix_trans(pack2<__half>(w[i][n][2], w[i][n][3]));
-        }
+    for (int n = 0; n < NQ; ++n) {
+        st.l[n][0] += pr[n][0] + pr[n][2];
+        st.l[n][1] += pr[n][1] + pr[n][3];
+        weight[n][0] = movmatrix_trans(pack2<__half>(w[n][0], w[n][1]));
+        weight[n][1] = movmatrix_trans(pack2<__half>(w[n][2], w[n][3]));
     }
     // ---- O^T += V^T P^T: lane (g, t) has codes 16 g .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
+    for (int c = 0; c < VG; ++c) {
+        uint4 v[4];
 #pragma unroll
-        for (int c = 0; c < VG; ++c) {
-            uint4 v[4];
+        for (int r = 0; r < 4; ++r) {
+            v[r] = *reinterpret_cast<const uint4*>(slot + c * at.line + (at.v[r / 2] ^ (r % 2 * 16)) + r % 2 * 128);
+        }
+        const uint32_t words[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
+                                      {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                v[r] = *reinterpret_cast<const uint4*>(slot[i] + c * at.line + (at.v[r / 2] ^ (r % 2 * 16)) + r % 2 * 128);
-            }
-            const uint32_t words[4][4] = {{v[0].x, v[0].y, v[0].z, v[0].w}, {v[1].x, v[1].y, v[1].z, v[1].w},
-                                          {v[2].x, v[2].y, v[2].z, v[2].w}, {v[3].x, v[3].y, v[3].z, v[3].w}};
+        for (int e = 0; e < 4; ++e) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int j = 0; j < 2; ++j) {
+                // bytes 2j, 2j + 1 of the four tokens: [byte][token pair]
+                uint32_t frag[4];
+                codes4_to_half<CODE>(__byte_perm(words[0][e], words[1][e], j == 0 ? 0x5140 : 0x7362), frag[0], frag[1]);
+                codes4_to_half<CODE>(__byte_perm(words[2][e], words[3][e], j == 0 ? 0x5140 : 0x7362), frag[2], frag[3]);
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    // bytes 2j, 2j + 1 of the four tokens: [byte][token pair]
-                    uint32_t frag[4];
-                    codes4_to_half<CODE>(__byte_perm(words[0][e], words[1][e], j == 0 ? 0x5140 : 0x7362), frag[0], frag[1]);
-                    codes4_to_half<CODE>(__byte_perm(words[2][e], words[3][e], j == 0 ? 0x5140 : 0x7362), frag[2], frag[3]);
-#pragma unroll
-                    for (int n = 0; n < NQ; ++n) mma_16816<__half>(st.acc[n][c * 8 + e * 2 + j], frag, weight[i][n][0], weight[i][n][1]);
-                }
+                for (int n = 0; n < NQ; ++n) mma_16816<__half>(st.acc[n][c * 8 + e * 2 + j], frag, weight[n][0], weight[n][1]);
             }
         }
     }
@@ -906,15 +877,13 @@ __device__ __forceinline__ void scaled_share(const MapParams& p, const ActiveCou
 }
 
 // ------------------------------ one share of tiles per warp ------------------------------------------------------
-// NT: tiles worked on side by side.
-template <typename T, int CODE, int D, int NQ, int W, int HP, int NT>
+template <typename T, int CODE, int D, int NQ, int W, int HP>
 __global__ void __launch_bounds__(W * 32, 1)
 sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_constant__ CUtensorMap, const MapParams p) {
     using G = ScaledGeometry<D, NQ, W, HP, true>;
     constexpr int S = G::kSlots;
     constexpr int U = G::kUnits;
     constexpr int KS = D / 16;
-    static_assert(S >= 2 * NT, "one group of tiles in work, one on its way");
 
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -1057,23 +1026,18 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
         fetch.begin = begin;
         fetch.end = end;
         uint32_t next = begin;  // tile to fetch
-        for (uint32_t x = begin; x < end;) {
+        for (uint32_t x = begin; x < end; ++x) {
             // a pair's slot is refilled one tile later, so that its first warp rarely waits for the second
             if (pair == 0) {
                 for (; ok && next < x + S - (HP - 1); ++next) ok = fetch.issue(next);
             }
-            uint8_t* slots[NT];
-            const uint8_t* scales[NT];
-            uint2 info[NT];
             ok = ok && mbar_wait(fetch.full_bar + 8 * slot, phase, abort_flag, p);
             if (!__all_sync(0xffffffffu, ok)) {
                 ok = false;
                 break;
             }
-            slots[0] = my_ring + slot * G::kSlotBytes;
-            scales[0] = my_scales + slot * G::kScaleBytes;
-            info[0] = my_infos[(x - begin) & 63];
-            const uint32_t tile_chain = (info[0].x >> 8) & 0xffu;
+            const uint2 info = my_infos[(x - begin) & 63];
+            const uint32_t tile_chain = (info.x >> 8) & 0xffu;
             if (tile_chain != chain) {
                 if (chain != 0xffffffffu) leave_chain();
                 chain = tile_chain;
@@ -1087,47 +1051,13 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
                     for (int c = 0; c < 2; ++c) st.factor[n][c] = __shfl_sync(0xffffffffu, factor, int(8 * t + 4 * c));
                 }
             }
-            auto q = [&](int n, int step) { return q_frag[n][step]; };
-            const uint32_t first_slot = slot;
-            auto advance = [&]() {
-                if (++slot == uint32_t(S)) {
-                    slot = 0;
-                    phase ^= 1;
-                }
-            };
-            advance();
-            bool two = false;
-            if constexpr (NT == 2) {
-                if (x + 1 < end) {
-                    ok = mbar_wait(fetch.full_bar + 8 * slot, phase, abort_flag, p);
-                    if (!__all_sync(0xffffffffu, ok)) {
-                        ok = false;
-                        break;
-                    }
-                    info[1] = my_infos[(x + 1 - begin) & 63];
-                    two = ((info[1].x >> 8) & 0xffu) == chain;
-                }
-                if (two) {
-                    slots[1] = my_ring + slot * G::kSlotBytes;
-                    scales[1] = my_scales + slot * G::kScaleBytes;
-                    uint8_t* const both[2] = {slots[0], slots[1]};
-                    const uint8_t* const both_scales[2] = {scales[0], scales[1]};
-                    scaled_tiles<CODE, D, NQ, 2, HP>(p, st, both, both_scales, info, items, pair, at, lane, q);
-                }
-            }
-            if (!two) {
-                uint8_t* const one[1] = {slots[0]};
-                const uint8_t* const one_scale[1] = {scales[0]};
-                const uint2 one_info[1] = {info[0]};
-                scaled_tiles<CODE, D, NQ, 1, HP>(p, st, one, one_scale, one_info, items, pair, at, lane, q);
-            }
+            scaled_tile<CODE, D, NQ, HP>(p, st, my_ring + slot * G::kSlotBytes, my_scales + slot * G::kScaleBytes, info, items, pair, at, lane,
+                                         [&](int n, int step) { return q_frag[n][step]; });
             __syncwarp();
-            if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * first_slot);
-            ++x;
-            if (two) {
-                if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * slot);
-                advance();
-                ++x;
+            if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * slot);
+            if (++slot == uint32_t(S)) {
+                slot = 0;
+                phase ^= 1;
             }
         }
         bool pending = false;  // the state is the start of a chain that later units' shares continue
@@ -1284,11 +1214,8 @@ sdpa_scaled_chain_kernel(const __grid_constant__ CUtensorMap kv_map, const __gri
                 ok = false;
                 break;
             }
-            uint8_t* const slots[1] = {my_ring + slot * G::kSlotBytes};
-            const uint8_t* const scales[1] = {my_scales + slot * G::kScaleBytes};
-            const uint2 info[1] = {my_infos[(x - begin) & 63]};
-            scaled_tiles<CODE, D, NQ, 1, 1>(p, st, slots, scales, info, items, 0, at, lane,
-                                            [&](int n, int step) { return q_frag[(n * KS + step) * 32 + lane]; });
+            scaled_tile<CODE, D, NQ, 1>(p, st, my_ring + slot * G::kSlotBytes, my_scales + slot * G::kScaleBytes, my_infos[(x - begin) & 63],
+                                        items, 0, at, lane, [&](int n, int step) { return q_frag[(n * KS + step) * 32 + lane]; });
             __syncwarp();
             if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * slot);
             if (++slot == uint32_t(S)) {

@@ -499,7 +499,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             const uint32_t out_lane = sub * G::kGroupBytes + row4 * 128 + (((2 * cc) ^ row4) << 4);
             const uint32_t line_stride = short_pages ? 1024 : 2048, half_stride = short_pages ? G::kRawBytes / 2 : 1024;
             const uint32_t scale_plane = short_pages ? 8 : 16, scale_half = short_pages ? 16 : 8;
-            uint32_t step = 0, unit = 0;  // running numbers
+            uint32_t step = 0;  // running number
             bool ok = true;
             for (uint32_t taken = 0; ok; ++taken) {
                 const uint32_t ts = taken & 1;
@@ -510,9 +510,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 if (lane == 0) mbar_arrive(task_empty + 8 * ts);
                 const uint32_t slots = end > first ? (end - first + 15) / 16 : 0;
                 const uint32_t units = steps * G::kChunks * 2;
-                // this warp's first unit of the task
-                for (uint32_t u = (warp - G::kSoftmaxWarps + G::kConverters - unit % G::kConverters) % G::kConverters; u < units && ok;
-                     u += G::kConverters) {
+                // (one unit of every step: a warp keeps its chunk of a step and its plane)
+                for (uint32_t u = warp - G::kSoftmaxWarps; u < units && ok; u += G::kConverters) {
                     const uint32_t x = u >> 1, plane = u & 1;
                     const uint32_t number = step + x / G::kChunks, stage = number % G::kStages, phase = (number / G::kStages) & 1;
                     const uint32_t raw_number = step * G::kChunks + x, slot = raw_number % G::kRawSlots;
@@ -585,7 +584,6 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     __syncwarp();
                     if (lane == 0) mbar_arrive((plane == 0 ? k_full : v_full) + 8 * stage);
                 }
-                unit += units;
                 step += steps;
             }
         }
