@@ -37,7 +37,7 @@ class Config:
         return out
 
     def num_tokens_per_page(self) -> int:
-        return self.page_bytes // (2 * self.num_kv_heads * self.head_dim * self.kv_element_dtype().item_size())
+        return self.page_bytes // (2 * self.num_kv_heads * self.kv_element_dtype().kv_row_bytes(self.head_dim))
 
     def q_heads_per_kv_head(self) -> int:
         return self.num_q_heads // self.num_kv_heads
