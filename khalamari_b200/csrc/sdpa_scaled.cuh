@@ -1036,6 +1036,8 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
                 ok = false;
                 break;
             }
+            uint8_t* const codes = my_ring + slot * G::kSlotBytes;
+            const uint8_t* const scales = my_scales + slot * G::kScaleBytes;
             const uint2 info = my_infos[(x - begin) & 63];
             const uint32_t tile_chain = (info.x >> 8) & 0xffu;
             if (tile_chain != chain) {
@@ -1051,14 +1053,14 @@ sdpa_scaled_stream_kernel(const __grid_constant__ CUtensorMap kv_map, const __gr
                     for (int c = 0; c < 2; ++c) st.factor[n][c] = __shfl_sync(0xffffffffu, factor, int(8 * t + 4 * c));
                 }
             }
-            scaled_tile<CODE, D, NQ, HP>(p, st, my_ring + slot * G::kSlotBytes, my_scales + slot * G::kScaleBytes, info, items, pair, at, lane,
-                                         [&](int n, int step) { return q_frag[n][step]; });
-            __syncwarp();
-            if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * slot);
+            const uint32_t first_slot = slot;  // (moving on before the tile is 3 % faster than after it: 64 decode sequences, int8)
             if (++slot == uint32_t(S)) {
                 slot = 0;
                 phase ^= 1;
             }
+            scaled_tile<CODE, D, NQ, HP>(p, st, codes, scales, info, items, pair, at, lane, [&](int n, int step) { return q_frag[n][step]; });
+            __syncwarp();
+            if (lane == 0) mbar_arrive(fetch.empty_bar + 8 * first_slot);
         }
         bool pending = false;  // the state is the start of a chain that later units' shares continue
         if (ok && chain != 0xffffffffu) {
