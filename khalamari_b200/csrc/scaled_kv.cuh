@@ -76,18 +76,14 @@ __device__ __forceinline__ void codes4_to_half(uint32_t word, uint32_t& lo, uint
 }
 
 // 2^(b - 127) as packed pairs of T, in two factors: f16 scales may lie below its smallest normal number, and the product
-// of a code with the first factor is exact. As an operand of P V (`v`) a bf16 row is taken 2^-kValueShift times its size,
-// for sums that stay inside f32 (rows below 2^-116 lose bits to that), and a row that is not finite counts as zeros (its
-// K is NaN, which is what reaches the queries that see it).
-constexpr uint32_t kValueShift = 10;
+// of a code with the first factor is exact. Where V's byte marks a row that is not finite its codes count as zeros (the
+// row's K is NaN, which is what reaches the queries that see it).
 template <typename T>
 __device__ __forceinline__ void scaled_factors(uint32_t b, bool v, uint32_t& first, uint32_t& second);
 template <>
 __device__ __forceinline__ void scaled_factors<__nv_bfloat16>(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
     if (v && b == 255) b = 0;
-    // (below 2^-126 a subnormal power)
-    const uint32_t power = !v ? b << 7 : b > kValueShift ? (b - kValueShift) << 7 : 0x80u >> (kValueShift + 1 - b);
-    first = power * 0x00010001u;
+    first = (b << 7) * 0x00010001u;
     second = 0;
 }
 template <>
@@ -102,6 +98,22 @@ __device__ __forceinline__ void scaled_factors<__half>(uint32_t b, bool v, uint3
     first = uint32_t((high + 15) << 10) * 0x00010001u;
     // (below 2^-14 a subnormal power; scales below 2^-38 leave nothing of a code either way)
     second = (rest >= -14 ? uint32_t((rest + 15) << 10) : 1u << (rest + 24)) * 0x00010001u;
+}
+
+// The same for operands of a product (sdpa_scaled_tc.cuh): bf16 rows are taken 2^-kOperandShift times their size, so that a row
+// of bf16's largest value (2^128 in codes) is finite. Rows below 2^-116 lose bits to that (their factor is subnormal).
+template <typename T>
+constexpr int kOperandShift = std::is_same<T, __nv_bfloat16>::value ? 10 : 0;
+template <typename T>
+__device__ __forceinline__ void operand_factors(uint32_t b, bool v, uint32_t& first, uint32_t& second) {
+    if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+        if (v && b == 255) b = 0;
+        // (the upper half of an f32 power is the bf16 one)
+        first = __byte_perm(__float_as_uint(__uint_as_float(b << 23) * (1.0f / (1 << kOperandShift<T>))), 0u, 0x3232);
+        second = 0;
+    } else {
+        scaled_factors<T>(b, v, first, second);
+    }
 }
 
 template <typename T>

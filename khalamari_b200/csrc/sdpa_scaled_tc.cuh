@@ -6,10 +6,10 @@
 //
 // Codes become 16-bit operands of the Q/output type once per step of 64 tokens, in shared memory, with their row's
 // power-of-two scale already applied: int8 and E4M3 codes times 2^e are exact in bf16, and in f16 as far as its range goes
-// (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). Every operand is finite where
-// the cache is: a hidden token's probability is 0, and 0 times an infinity would not be. O sums up to 2^8 |v| for each token,
-// which for rows at the top of bf16's range leaves f32; bf16 V operands are 2^-10 of their size, and the epilogue takes that
-// back. At head_dim 128 two Q tiles of
+// (results are rounded below 2^-14 and saturate at 65504, as values of an f16 cache would). Operands are finite where the
+// cache is: a hidden token's probability is 0, and 0 times an infinity would not be. So bf16 operands are 2^-10 of their size
+// (2^128, what codes of bf16's largest value stand for, is beyond its range), which the scale of the scores and the epilogue
+// take back; it also keeps O, a sum of up to 2^8 |v| for each token, inside f32 for such rows. At head_dim 128 two Q tiles of
 // the same sequence and KV head share every converted step (at 256 tensor memory holds the output of one). A probability
 // is rounded to the Q/output type: in bf16 that is off by at most 2^-8, no more than what the cache rounds off a V element
 // (2^-8 to 2^-7 of the row's largest).
@@ -550,9 +550,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         }
                     }
                     uint8_t* const out = (plane == 0 ? k_ring : v_ring) + stage * G::kOperandBytes + (x % G::kChunks) * 2048;
-                    // values beyond T's largest (bf16's V rows are shifted down instead)
                     bool cut = false;
-                    if (std::is_same<T, __half>::value || plane == 0) {
+                    if constexpr (std::is_same<T, __half>::value) {
                         bool large = false;
 #pragma unroll
                         for (int i = 0; i < 4; ++i) large = large || (b[i] >= first_large_byte<T>() && b[i] < 255);
@@ -561,7 +560,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t one, two;
-                        scaled_factors<T>(b[i], plane == 1, one, two);
+                        operand_factors<T>(b[i], plane == 1, one, two);
 #pragma unroll
                         for (int line = 0; line < G::kLines; ++line) {
                             const uint4 w4 = words[line][i];
@@ -569,8 +568,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                             uint32_t r[8];
 #pragma unroll
                             for (int w = 0; w < 4; ++w) decode4<T, CODE>(raw_words[w], one, two, r[2 * w], r[2 * w + 1]);
-                            if (cut) {
-                                // (2^16, or 2^128, is the one value past T's largest that a code of a T row stands for)
+                            if (std::is_same<T, __half>::value && cut) {
+                                // (2^16 is the one value past f16's largest that a code of an f16 row stands for)
 #pragma unroll
                                 for (int w = 0; w < 8; ++w) r[w] = saturate2<T>(r[w]);
                             }
@@ -594,6 +593,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
         const uint32_t row = quad * 32 + lane;
         const uint32_t lane_base = (quad * 32) << 16;
         const uint32_t o_at = tmem_o + 128 * tile + lane_base;
+        const float scale_log2e = p.scale_log2e * float(1 << kOperandShift<T>);
         uint32_t mine = 0, done_tasks = 0;  // running numbers of this tile: steps, tasks
         bool ok = true;
         for (uint32_t taken = 0; ok; ++taken) {
@@ -656,9 +656,9 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                 }
                 const float top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
                 // lazy maximum: moved (with the sum and O) only when the step exceeds it by more than 2^8
-                const bool grow = top > -INFINITY && (m == -INFINITY || (top - m) * p.scale_log2e > kRescaleLog2);
+                const bool grow = top > -INFINITY && (m == -INFINITY || (top - m) * scale_log2e > kRescaleLog2);
                 if (__any_sync(0xffffffffu, grow)) {
-                    const float keep = grow && m != -INFINITY ? fast_exp2((m - top) * p.scale_log2e) : 1.0f;
+                    const float keep = grow && m != -INFINITY ? fast_exp2((m - top) * scale_log2e) : 1.0f;
                     if (grow) {
                         l *= keep;
                         m = top;
@@ -682,8 +682,8 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                         tmem_st_wait();
                     }
                 }
-                const float shift = m == -INFINITY ? 0.0f : -m * p.scale_log2e;
-                const float2 scale2 = make_float2(p.scale_log2e, p.scale_log2e), shift2 = make_float2(shift, shift);
+                const float shift = m == -INFINITY ? 0.0f : -m * scale_log2e;
+                const float2 scale2 = make_float2(scale_log2e, scale_log2e), shift2 = make_float2(shift, shift);
                 float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                 for (int c = 0; c < G::kStep; c += 32) {
@@ -708,8 +708,7 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
             // ---- epilogue
             // (a token that is seen adds 1 at the maximum, unless every score is -inf: that softmax is NaN)
             if (l == 0.0f && hi > lo) l = __uint_as_float(0x7fc00000u);
-            constexpr float kUnshift = std::is_same<T, __nv_bfloat16>::value ? float(1u << kValueShift) : 1.0f;
-            const float inv = l == 0.0f ? 0.0f : kUnshift / l;  // (a NaN sum stays NaN)
+            const float inv = l == 0.0f ? 0.0f : float(1 << kOperandShift<T>) / l;  // (a NaN sum stays NaN)
             const uint64_t index = (uint64_t(tmpl) * p.num_q_heads + head) * p.max_q_tokens + row_tok;
             if (steps > 0) {
                 ok = mbar_wait_warp(o_full + 8 * tile, done_tasks & 1, abort_flag, p);
@@ -728,30 +727,20 @@ sdpa_scaled_tc_kernel(const __grid_constant__ CUtensorMap kv_map, const __grid_c
                     for (int i = 0; i < 32; ++i) o[i] = 0u;
                 }
                 // (averages of largest values: rounded probabilities can take them a step too far)
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const float x = __uint_as_float(o[i]) * inv;
-                    o[i] = __float_as_uint(p.direct != 0 ? saturate<T>(x) : saturate<__nv_bfloat16>(x));
-                }
                 if (valid && p.direct != 0) {
                     T* const dst = static_cast<T*>(p.out) + q_row * D + c;
+                    auto pair = [&](int i) { return saturate2<T>(pack2<T>(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv)); };
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 v;
-                        v.x = pack2<T>(__uint_as_float(o[i]), __uint_as_float(o[i + 1]));
-                        v.y = pack2<T>(__uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                        v.z = pack2<T>(__uint_as_float(o[i + 4]), __uint_as_float(o[i + 5]));
-                        v.w = pack2<T>(__uint_as_float(o[i + 6]), __uint_as_float(o[i + 7]));
-                        *reinterpret_cast<uint4*>(dst + i) = v;
-                    }
+                    for (int i = 0; i < 32; i += 8) *reinterpret_cast<uint4*>(dst + i) = make_uint4(pair(i), pair(i + 2), pair(i + 4), pair(i + 6));
                 } else if (valid) {
                     float* const dst = p.partial_out + index * D + c;
+                    auto one = [&](int i) { return saturate<__nv_bfloat16>(__uint_as_float(o[i]) * inv); };
 #pragma unroll
-                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<uint4*>(dst + i) = make_uint4(o[i], o[i + 1], o[i + 2], o[i + 3]);
+                    for (int i = 0; i < 32; i += 4) *reinterpret_cast<float4*>(dst + i) = make_float4(one(i), one(i + 1), one(i + 2), one(i + 3));
                 }
             }
             if (valid && p.direct == 0) {
-                publish_partial_stats(p.partial_sum, p.partial_max, index, m * (p.scale_log2e * 0.6931471805599453f), l);
+                publish_partial_stats(p.partial_sum, p.partial_max, index, m * (scale_log2e * 0.6931471805599453f), l);
             }
             if (steps > 0) {
                 tmem_fence_before();
