@@ -528,11 +528,10 @@ __device__ __forceinline__ float scaled_load_q(const MapParams& p, const ScaledR
     if (most >= kInfinity) {
         factor = __uint_as_float(0x7fc00000u);  // a NaN or an infinity: all scores of the row are NaN or infinite
     } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-        const int exponent = int(most >> 7);  // of the largest element, biased
-        if (exponent >= 9) {                  // (tinier rows go as they are)
-            up = __uint_as_float(uint32_t(262 - exponent) << 23);  // 2^(8 - k), k = exponent - 127
-            factor = p.scale_log2e * __uint_as_float(uint32_t(exponent - 8) << 23);
-        }
+        // of the largest element, biased (rows below 2^-111 stay below 2^8, so that the factor is no subnormal)
+        const int exponent = max(int(most >> 7), 16);
+        up = __uint_as_float(uint32_t(262 - exponent) << 23);  // 2^(8 - k), k = exponent - 127
+        factor = p.scale_log2e * __uint_as_float(uint32_t(exponent - 8) << 23);
     }
 #pragma unroll
     for (int c = 0; c < KC; ++c) {

@@ -91,3 +91,19 @@ def test_scores_that_rise_within_a_factor_before_the_largest_rows(device, code, 
     # one distinct query: the reference of one head a KV head serves the group
     expected, bound = reference(case)
     assert_close(out, expected, bound)
+
+
+@pytest.mark.parametrize("code", CODES)
+@pytest.mark.parametrize("power", [-122, -60, 100])
+@pytest.mark.parametrize("hq,hkv,d,histories,q_lens", [
+    (16, 2, 128, [300, 33], [1, 1]), (24, 2, 256, [300, 33], [1, 1]), (24, 4, 256, [90], [4]), (16, 2, 128, [300], [64]), (16, 2, 256, [300], [64]),
+])
+def test_rows_of_q_and_k_whose_sizes_cancel(device, code, power, hq, hkv, d, histories, q_lens):
+    """Q of size 2^power against K of size 2^(-1 - power): the scores are ordinary, the operands reach both ends of bf16's range."""
+    case = make_scaled_case(17, code, "bf16", hq, hkv, d, histories, q_lens)
+    case.q_bits[:] = round_to("bf16", (bits_to_f32("bf16", case.q_bits) * np.float32(2.0 ** power)).astype(np.float32))[0].reshape(case.q_bits.shape)
+    for r, k in enumerate(case.k):
+        _put(case, r, np.arange(len(k)), k=k * 2.0 ** (-1 - power))
+    run = ScaledRun(device, case, max_tokens=256)
+    out = run.run()
+    assert_close(out, *reference(case, wide=run.wide()))
