@@ -69,7 +69,11 @@ enum {
      * A page holds [K/V][Hkv][P][D] code bytes and behind them [Hkv][K/V][P] scale bytes b, so page_bytes =
      * 2 * Hkv * P * (D + 1). A row stands for code * 2^(b - 127); b = 0 marks a row of zeros, and b = 255 a token
      * whose K or V row (of that KV head) held a NaN or an infinity: both rows then hold zero codes, read back as NaN
-     * and give NaN to every query that sees the token. Head dimensions 128 and 256, pages of 8, 16 or 32 tokens. */
+     * and give NaN to every query that sees the token. Head dimensions 128 and 256, pages of 8, 16 or 32 tokens (32 at
+     * head_dim 128: attention takes new tokens one by one). Attention gives NaN to a Q row that is not finite. Tasks of
+     * up to 32 Q rows (24 at head_dim 256) multiply the codes themselves; wider ones round the rows to the Q/output type
+     * first, so that with Float16 they saturate at 65504 and lose bits below 2^-14: pages written from Bfloat16 may hold
+     * rows that Float16 queries see differently in decode and in prefill. */
     KH_DTYPE_INT8_SCALED = 101,      /* two's complement codes in [-127, 127] */
     KH_DTYPE_FP8_E4M3FN_SCALED = 102 /* FP8 E4M3FN codes, the row's largest magnitude in (224, 448] */
 };
@@ -343,10 +347,11 @@ KH_API kh_status kh_metadata_update(const kh_metadata_arrays* arrays, const uint
  * kv_dtype = KH_DTYPE_FP8_E4M3FN: the reference's cache format; codes are decoded on load exactly as
  * metal/gqa_fp8.metal:1-25 does (16-token pages, head_dim 128 or 256). kv_dtype = dtype: the pages hold
  * Q/output-type elements. kv_dtype = KH_DTYPE_INT8_SCALED / KH_DTYPE_FP8_E4M3FN_SCALED: codes with a scale byte for
- * each (token, KV head) row (every (head_dim, tokens_per_page) profile; kv_pages and q 16-byte aligned; the
- * one-launch map + reduce form is not offered). Their partials carry an exp sum of 1 under the logarithm of the whole sum
- * as maximum (0 and -inf where nothing is visible; NaN and 0 where a score is NaN), which any merge takes as it takes the
- * others. Outputs saturate at the type's largest finite value, as the page read's do. */
+ * each (token, KV head) row (kv_pages and q 16-byte aligned; the one-launch map + reduce form is not offered; select
+ * with KH_POLICY_B200_CHAINED, whose slices fit these kernels). Their partials carry an exp sum of 1 under the logarithm
+ * of the whole sum as maximum (0 and -inf where nothing is visible; NaN and 0 where a score is NaN), which any merge takes
+ * as it takes the others. Outputs of the direct form and of the reduce saturate at the type's largest finite value, as the
+ * page read's do. */
 typedef struct kh_sliced_kv_config {
     uint32_t num_q_heads;
     uint32_t num_kv_heads;

@@ -29,7 +29,7 @@ static MapInstance make_tc_instance() {
 }
 
 // Accumulators take D / 16 x NQ x 4 registers of a thread, which sets the warps per SM; wider tasks go to tcgen05, whose
-// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 496 us here, 856 us there). `paired`: the
+// tiles of 128 rows cost the same however few are used (24 rows at head_dim 256: 500 us here, 856 us there). `paired`: the
 // KV heads can be taken two at a time (64 decode sequences: 145 us, one at a time 150 us).
 template <typename T, int CODE, int D>
 static MapInstance pick_scaled_rows(uint32_t rows, bool paired) {

@@ -9,9 +9,11 @@
 //
 // Two running references per Q row, both raised lazily (only when exceeded by 2^8): m for the scores, which the sum
 // is relative to, and r for score + eV (all in the log2 domain), which the value weights w_t = 2^(s_t + eV_t - r) are
-// relative to. A weight is then at most 2^8 whatever the V scales are, and rounding it to f16 costs at most 2^-12 of
-// the term it multiplies; one reference for both would push the weights of tokens with small V rows out of f16's
-// range. The output is O * 2^(r - m) / l.
+// relative to. A weight is then at most 2^8 whatever the V scales are. Rounding it to f16 costs at most 2^-11 of the term it
+// multiplies for weights from 2^-14 on, and 2^-25 for smaller ones (those below 2^-25 vanish, while the sum counts their
+// probability): n tokens far below a dominant one lose at most n 2^-25 of its term, n being the tokens of one warp's share.
+// One reference for both would push the weights of tokens with small V rows out of f16's range. The output is
+// O * 2^(r - m) / l.
 //
 // K and V codes of a 16-token tile arrive by TMA (128-byte swizzle), its scale bytes by a small bulk copy, on one
 // mbarrier per slot of a ring that belongs to one warp, or to a pair of warps that work on neighbouring KV heads of the
@@ -33,11 +35,11 @@
 //    wide to park one for every warp beside the staging ring.
 //
 // What bounds them: at head_dim 128 the copies alone would take 107 us for 64 decode sequences of 1,024-8,192 tokens (64 / 8
-// heads, 604 MB of codes and scales), the step takes 138-140 us with int8 codes (4.3 TB/s) and 123-127 us with E4M3 (4.8 TB/s),
-// its reduce included: 440 warp instructions per 16-token int8 tile and head, which 12 warps do not hide altogether. 16
-// warps with two slots each took 148 us, 8 warps 160. At head_dim 256, 24 rows (32 sequences of four verify tokens, 24 / 4
-// heads, 1.35 GB): 496 us, 2.7 TB/s; 192 accumulator registers a thread leave two warps a scheduler, which wait for fixed
-// latencies. One sequence of 524,288 tokens (16 / 2 heads, 256): 119 us, 4.5 TB/s.
+// heads, 604 MB of codes and scales), the step takes 135-140 us with int8 codes (4.3-4.5 TB/s) and 125-130 us with E4M3
+// (4.7 TB/s), its reduce included: 440 warp instructions per 16-token int8 tile and head, which 12 warps do not hide
+// altogether. 16 warps with two slots each took 148 us, 8 warps 160. At head_dim 256, 24 rows (32 sequences of four verify
+// tokens, 24 / 4 heads, 1.35 GB): 500 us, 2.7 TB/s; 192 accumulator registers a thread leave two warps a scheduler, which
+// wait for fixed latencies. One sequence of 524,288 tokens (16 / 2 heads, 256): 117-120 us, 4.5 TB/s, by the same 8 warps.
 #pragma once
 
 #include "scaled_kv.cuh"

@@ -22,10 +22,13 @@
 // conversion have to keep ahead of that, which takes eight conversion warps (a unit of 16 rows takes 650 cycles, nearly all
 // of them latency) and two copy warps (one warp issues a copy and its scale bytes every 660 cycles).
 //
-// Four sequences of 2,048 new tokens behind contexts of 2,048 to 12,288 (64 / 8 heads, head_dim 128, bf16, int8): 1,750 us,
-// 810 TFLOP/s. Two of 2,048 behind 4,000 at head_dim 256 (32 / 4 heads): 894 us, 740 TFLOP/s, bound by the conversion, which has
-// 64 raw tokens in flight. 517 tokens at head_dim 256 (16 / 2 heads, f16, E4M3): 38-39 us with the reduce. (Q rows loaded and O
-// rows stored a row per thread: whole rows at a time, with the rows' addresses shuffled, was 5 % slower.)
+// Four sequences of 2,048 new tokens behind contexts of 2,048 to 12,288 (64 / 8 heads, head_dim 128, bf16, int8): 1,740 us
+// back to back, 815 TFLOP/s (1,660 us after a pause). No one part bounds it: without the exponentials it is 10 % shorter,
+// without the codes' conversion 4 %, without both products 9 %, without all three 34 %; the rest is the hand-over from warp to
+// warp in every step. Two of 2,048 behind 4,000 at head_dim 256 (32 / 4 heads): 904 us, 735 TFLOP/s; there the conversion's
+// instructions are 14 %, the products 16 %, the exponentials 1 %, and the three together 32 %. 517 tokens at head_dim 256
+// (16 / 2 heads, f16, E4M3): 37-39 us with the reduce, of which those parts are 4. (Q rows loaded and O rows stored a row per
+// thread: whole rows at a time, with the rows' addresses shuffled, was 5 % slower.)
 //
 // Warps: softmax and epilogue, one thread a row (0-3 tile A, 4-7 tile B), conversion (8), tensor-core issue (one lane, a
 // warp for each tile), task decoding and copies (2). All waits are bounded (mbar_wait); no named barriers between roles.
